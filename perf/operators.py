@@ -5,11 +5,13 @@ A case is one pass as a training step (forward, then every gradient) or a valida
 it.  With `own` set, `run` calls the framework's operators; otherwise it computes the same values from elementary torch
 operations in 32 bits.  `exact` computes them in 64 bits.
 
-    dropout                y[i] = x[i] * [word(i // run) >= round(p * 2^32)] / (1 - p),  word(j) = word j % 4 of
-                           Philox4x32-10(counter = (j // 4, offset), key = seed), run = elements that share a draw
+    dropout                y[i] = x[i] * [draw(i // run) >= round(p * 2^32)] / (1 - p), run = elements that share a draw.
+                           Philox4x32-10(counter = (j // 8, offset), key = seed) gives the upper 16 bits of the draws 8 (j // 8)
+                           ... + 7, low halves of its words first; the lower 16 bits come from the counter j // 8 + 2^63
     linear_cross_entropy   z = x W^T + b,  loss_t = logsumexp(z_t) - (1 - s) z_t[y_t] - s mean(z_t), averaged or summed
                            over the rows that are not ignored, or one by one
 """
+import functools
 import math
 import os
 import sys
@@ -108,18 +110,13 @@ def prepare(case, seed):
         return (torch.randn(*shape, device="cuda", generator=gen) * std).to(dtype)
 
     st = dict(case)
-    if own:
-        sys.path[:0] = [p for p in [os.path.abspath("deformable-kernels_b200")] if p not in sys.path]
-        from deformable_kernels.ops.deform_kernel import functions
-        st["call"] = functions.dropout if case["op"] == "dropout" else functions.linear_cross_entropy
     if case["op"] == "dropout":
         shape = _shape(case)
         st["x"] = normal(*shape)
         st["dy"] = normal(*shape) if case["grad"] else None
         # what a training program keeps on the device: the seed and the number of the draw
         st["state"] = torch.tensor([seed * 0x9E3779B97F4A7C15 % (1 << 63), 1000 + seed % 1000], device="cuda", dtype=torch.int64)
-        if own:
-            st["x"].requires_grad_(case["grad"])
+        st["x"].requires_grad_(case["grad"])
         return st
     t, d, v = case["rows"], case["features"], case["classes"]
     w = normal(v, d, std=1.5 / math.sqrt(d))
@@ -142,33 +139,37 @@ def prepare(case, seed):
         elif case["reduction"] == "sum":
             up = up / t
         st["up"] = up
-    if own:
-        for k in ("x", "w", "b"):
-            if st[k] is not None:
-                st[k].requires_grad_(case["grad"])
+    for k in ("x", "w", "b"):
+        if st[k] is not None:
+            st[k].requires_grad_(case["grad"])
     return st
 
 
-def _philox_words(count, state):
-    """The first `count` random words, in int64: ten rounds on counters (group, offset) under the key `seed`."""
+def _philox(group, state):
+    """Ten rounds on the counters (group, offset) under the key `seed`: eight half words a counter, in int64."""
     low = 0xFFFFFFFF
-    group = torch.arange((count + 3) // 4, device=state.device, dtype=torch.int64)
     zero = torch.zeros_like(group)
-    c0, c1 = group & low, group >> 32
+    c0, c1 = group & low, (group >> 32) & low
     c2, c3 = zero + (state[1] & low), zero + ((state[1] >> 32) & low)
     k0, k1 = state[0] & low, (state[0] >> 32) & low
     for _ in range(10):
         a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57     # modulo 2^64, which holds the whole product
         c0, c1, c2, c3 = ((b >> 32) & low) ^ c1 ^ k0, b & low, ((a >> 32) & low) ^ c3 ^ k1, a & low
         k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
-    return torch.stack([c0, c1, c2, c3], 1).view(-1)[:count]
+    words = torch.stack([c0, c1, c2, c3], 1)
+    return torch.stack([words & 0xFFFF, words >> 16], 2).view(-1)
+
+
+def _draws(count, state):
+    group = torch.arange((count + 7) // 8, device=state.device, dtype=torch.int64)
+    return ((_philox(group, state) << 16) | _philox(group | -(1 << 63), state))[:count]
 
 
 def _plain_dropout(st):
     x = st["x"]
     shared = st["shared_dims"]
     lead = x.shape[:x.dim() - shared]
-    keep = (_philox_words(math.prod(lead), st["state"]) >= int(math.floor(st["p"] * 2.0 ** 32 + 0.5))).view(*lead, *[1] * shared)
+    keep = (_draws(math.prod(lead), st["state"]) >= int(math.floor(st["p"] * 2.0 ** 32 + 0.5))).view(*lead, *[1] * shared)
     scale = 1.0 / (1.0 - st["p"])
     zero = torch.zeros((), device=x.device)
     y = torch.where(keep, x.float() * scale, zero).to(x.dtype)
@@ -212,8 +213,15 @@ def _plain_head(st):
     return out
 
 
+@functools.lru_cache(maxsize=None)
+def _functions():
+    sys.path[:0] = [p for p in [os.path.abspath("deformable-kernels_b200")] if p not in sys.path]
+    from deformable_kernels.ops.deform_kernel import functions
+    return functions
+
+
 def _own_dropout(st):
-    dropout = st["call"]
+    dropout = _functions().dropout
     if not st["grad"]:
         with torch.no_grad():
             return {"y": dropout(st["x"], st["p"], st["state"], shared_dims=st["shared_dims"])}
@@ -222,7 +230,7 @@ def _own_dropout(st):
 
 
 def _own_head(st):
-    linear_cross_entropy = st["call"]
+    linear_cross_entropy = _functions().linear_cross_entropy
     kw = dict(bias=st["b"], ignore_index=_IGNORE, reduction=st["reduction"], label_smoothing=st["smoothing"])
     if not st["grad"]:
         with torch.no_grad():
@@ -260,18 +268,21 @@ def _exact_keep(count, seed, offset, p, device):
         mid = (a >> 16) + (b & 0xFFFFFFFFFFFF)       # b < 2^48: the sum of the upper parts, below 2^49
         return mid >> 16, ((mid & 0xFFFF) << 16) | (a & 0xFFFF)
 
-    n = -(-count // 4)
+    n = -(-count // 8)
     index = torch.arange(n, device=device, dtype=torch.int64)
-    words = [index % (1 << 32), index // (1 << 32), torch.full_like(index, offset % (1 << 32)), torch.full_like(index, offset >> 32)]
-    for r in range(10):
-        h0, l0 = product(words[0], 0xD2511F53)
-        h1, l1 = product(words[2], 0xCD9E8D57)
-        key = ((seed % (1 << 32)) + r * 0x9E3779B9) % (1 << 32), ((seed >> 32) + r * 0xBB67AE85) % (1 << 32)
-        words = [h1 ^ words[1] ^ key[0], l1, h0 ^ words[3] ^ key[1], l0]
-    keep = torch.empty(n, 4, device=device, dtype=torch.bool)
-    for i in range(4):
-        keep[:, i] = words[i] >= round(p * (1 << 32))
-    return keep.flatten()[:count]
+    draws = torch.zeros(n, 8, device=device, dtype=torch.int64)
+    for part in range(2):
+        words = [index % (1 << 32), index // (1 << 32) + part * (1 << 31),
+                 torch.full_like(index, offset % (1 << 32)), torch.full_like(index, offset >> 32)]
+        for r in range(10):
+            h0, l0 = product(words[0], 0xD2511F53)
+            h1, l1 = product(words[2], 0xCD9E8D57)
+            key = ((seed % (1 << 32)) + r * 0x9E3779B9) % (1 << 32), ((seed >> 32) + r * 0xBB67AE85) % (1 << 32)
+            words = [h1 ^ words[1] ^ key[0], l1, h0 ^ words[3] ^ key[1], l0]
+        for i in range(8):
+            half = (words[i // 2] // (1 << 16 * (i % 2))) % (1 << 16)
+            draws[:, i] += half * (1 << 16 * (1 - part))
+    return (draws >= round(p * (1 << 32))).flatten()[:count]
 
 
 def exact(case, seed):
