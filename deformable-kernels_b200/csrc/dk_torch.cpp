@@ -47,6 +47,11 @@ using torch::autograd::variable_list;
   X(dk_global_dk_backward)                         \
   X(dk_offset_clip_forward)                        \
   X(dk_offset_clip_backward)                       \
+  X(dk_dropout)                                    \
+  X(dk_linear_cross_entropy_forward_workspace_bytes) \
+  X(dk_linear_cross_entropy_forward)               \
+  X(dk_linear_cross_entropy_backward_workspace_bytes) \
+  X(dk_linear_cross_entropy_backward)              \
   X(dk_status_string)                              \
   X(dk_last_cuda_error)
 
@@ -577,6 +582,182 @@ Tensor clip_offsets(const Tensor& offsets, const Tensor& bias, double lo, double
   return out;
 }
 
+// ------------------------------------------------------------------ classifier head
+
+// the head's operators take bfloat16 as well
+inline int head_dtype_code(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? DK_BF16 : dtype_code(t); }
+
+inline Tensor arrived_as(const variable_list& grads, at::IntArrayRef sizes, const at::TensorOptions& options) {
+  if (!grads[0].defined()) return at::zeros(sizes, options);
+  const Tensor& g = grads[0];
+  TORCH_CHECK_NOT_IMPLEMENTED(g.is_cuda(), "deformable kernels run on CUDA tensors only");
+  return g.to(options.dtype()).contiguous();
+}
+
+struct DropoutBackward : public Node {
+  Tensor used;  // seed and offset of the forward call, where they came from the device; not visible outside
+  bool on_device = false;
+  unsigned long long seed = 0, offset = 0;
+  double p = 0;
+  int64_t run = 1;
+  std::vector<int64_t> sizes;
+  at::TensorOptions options;
+
+  variable_list apply(variable_list&& grads) override {
+    at::NoGradGuard no_grad;
+    TORCH_CHECK(!on_device || used.defined(), "Trying to backward through the graph a second time");
+    const c10::DeviceGuard guard(options.device());
+    const Tensor dy = arrived_as(grads, sizes, options);
+    Tensor dx = empty_as(dy, sizes);
+    check(lib.dk_dropout(cptr(dy), mptr(dx), dy.numel(), run, p, seed, on_device ? 0 : offset, cptr(used), nullptr, head_dtype_code(dy),
+                         stream_of(dy)),
+          "dropout backward");
+    return {dx};
+  }
+  std::string name() const override { return "DropoutFunctionBackward"; }
+  void release_variables() override { used.reset(); }
+};
+
+// `state`: [seed, offset] on the device, or undefined: the two numbers
+Tensor dropout(const Tensor& input, double p, const Tensor& state, unsigned long long seed, unsigned long long offset,
+               int64_t shared_dims) {
+  require_cuda({&input, &state});
+  same_device(input, {&state});
+  no_forward_ad({&input});
+  TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "dropout probability has to be between 0 and 1, but got ", p);
+  TORCH_CHECK_VALUE(shared_dims >= 0 && shared_dims <= input.dim(), "shared_dims must be between 0 and the input's dimensions");
+  if (state.defined()) {
+    TORCH_CHECK_TYPE(state.scalar_type() == at::kLong, "the seed tensor must be int64, got ", state.scalar_type());
+    TORCH_CHECK_VALUE(state.numel() == 2, "the seed tensor holds two values, seed and offset");
+  }
+  const int code = head_dtype_code(input);
+  const bool grad = wants_grad({&input}) && input.numel() > 0;
+  int64_t run = 1;
+  for (int64_t d = input.dim() - shared_dims; d < input.dim(); ++d) run *= input.size(d);
+  Tensor out, used;
+  {
+    at::NoGradGuard no_grad;
+    const c10::DeviceGuard guard(input.device());
+    const Tensor x = input.contiguous();
+    out = empty_as(x, x.sizes());
+    if (x.numel() > 0) {
+      const Tensor st = state.defined() ? state.contiguous() : Tensor();
+      if (grad && st.defined()) used = empty_of(x, {2}, at::kLong);
+      check(lib.dk_dropout(cptr(x), mptr(out), x.numel(), run, p, seed, offset, cptr(st), mptr(used), code, stream_of(x)), "dropout forward");
+    }
+  }
+  if (grad) {
+    auto node = std::make_shared<DropoutBackward>();
+    node->set_next_edges(collect_next_edges(input));
+    node->used = used, node->on_device = used.defined();
+    node->seed = seed, node->offset = offset, node->p = p, node->run = run;
+    node->sizes = out.sizes().vec(), node->options = out.options();
+    torch::autograd::set_history(out, node);
+  }
+  return out;
+}
+
+struct CrossEntropyArgs {
+  int64_t ignore_index;
+  int reduction;
+  double smoothing;
+};
+
+// what the kernels take: dense, beginning on 16 bytes
+inline Tensor aligned(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.const_data_ptr()) & 15 ? c.clone() : c;
+}
+
+struct LinearCrossEntropyBackward : public Node {
+  SavedVariable input, weight, bias, target;
+  Tensor saved;  // log-sum-exp of the rows and their count; not visible outside
+  bool has_bias = false;
+  CrossEntropyArgs a;
+  std::vector<int64_t> in_sizes, out_sizes;
+
+  variable_list apply(variable_list&& grads) override {
+    at::NoGradGuard no_grad;
+    const Tensor x = input.unpack(), w = weight.unpack(), y = target.unpack(), b = has_bias ? bias.unpack() : Tensor();
+    TORCH_CHECK(saved.defined(), "Trying to backward through the graph a second time");
+    const c10::DeviceGuard guard(x.device());
+    const Tensor up = arrived_as(grads, out_sizes, saved.options());
+    Tensor dx, dw, db;
+    if (task_should_compute_output(0)) dx = empty_as(x, in_sizes);
+    if (task_should_compute_output(1)) dw = empty_as(w, w.sizes());
+    if (has_bias && task_should_compute_output(2)) db = empty_as(b, b.sizes());
+    const int rows = (int)y.numel(), features = (int)w.size(1), classes = (int)w.size(0);
+    if (rows == 0) {
+      if (dw.defined()) dw.zero_();
+      if (db.defined()) db.zero_();
+      return {dx, dw, db, Tensor()};
+    }
+    const int code = head_dtype_code(x);
+    const size_t bytes = lib.dk_linear_cross_entropy_backward_workspace_bytes(rows, features, classes, code);
+    Tensor ws = workspace(bytes, x);
+    check(lib.dk_linear_cross_entropy_backward(cptr(up), cptr(x), cptr(w), cptr(b), (const long long*)cptr(y), cptr(saved), mptr(dx),
+                                               mptr(dw), mptr(db), rows, features, classes, a.ignore_index, a.reduction, a.smoothing, code,
+                                               mptr(ws), bytes, stream_of(x)),
+          "linear_cross_entropy backward");
+    return {dx, dw, db, Tensor()};
+  }
+  std::string name() const override { return "LinearCrossEntropyFunctionBackward"; }
+  void release_variables() override {
+    input.reset_data(), weight.reset_data(), bias.reset_data(), target.reset_data();
+    saved.reset();
+  }
+};
+
+Tensor linear_cross_entropy(const Tensor& input, const Tensor& weight, const Tensor& target, const Tensor& bias,
+                            const CrossEntropyArgs& a) {
+  require_cuda({&input, &weight, &target, &bias});
+  same_dtype(input, {&weight, &bias});
+  same_device(input, {&weight, &target, &bias});
+  no_forward_ad({&input, &weight, &bias});
+  TORCH_CHECK_TYPE(target.scalar_type() == at::kLong, "target must be int64, got ", target.scalar_type());
+  TORCH_CHECK_VALUE(input.dim() >= 1 && weight.dim() == 2 && weight.size(1) == input.size(-1),
+                    "expected input [..., features] and weight [classes, features], got ", input.sizes(), " and ", weight.sizes());
+  TORCH_CHECK_VALUE(weight.size(0) > 0 && weight.size(1) > 0, "linear_cross_entropy needs at least one class and one feature");
+  TORCH_CHECK_VALUE(target.sizes() == input.sizes().slice(0, input.dim() - 1), "target must have the shape of input without its last dimension, got ",
+                    target.sizes(), " for ", input.sizes());
+  TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == weight.size(0)), "bias must have one entry per class");
+  TORCH_CHECK_VALUE(a.smoothing >= 0.0 && a.smoothing <= 1.0, "label_smoothing must be between 0 and 1, got ", a.smoothing);
+  const int code = head_dtype_code(input);
+  const bool grad = wants_grad({&input, &weight, &bias});
+  const int rows = as_int(target.numel()), features = as_int(weight.size(1)), classes = as_int(weight.size(0));
+  Tensor out, x, w, y, b, saved;
+  {
+    at::NoGradGuard no_grad;
+    const c10::DeviceGuard guard(input.device());
+    x = aligned(input), w = aligned(weight), y = target.contiguous();
+    if (bias.defined()) b = bias.contiguous();
+    const at::ScalarType type = code == DK_F64 ? at::kDouble : at::kFloat;
+    out = empty_of(x, a.reduction == DK_REDUCE_NONE ? target.sizes() : at::IntArrayRef(), type);
+    if (grad) saved = empty_of(x, {(int64_t)rows + 2}, type);
+    if (rows > 0) {
+      const size_t bytes = lib.dk_linear_cross_entropy_forward_workspace_bytes(rows, features, classes, code);
+      Tensor ws = workspace(bytes, x);
+      check(lib.dk_linear_cross_entropy_forward(cptr(x), cptr(w), cptr(b), (const long long*)cptr(y), mptr(out), mptr(saved), rows,
+                                                features, classes, a.ignore_index, a.reduction, a.smoothing, code, mptr(ws), bytes,
+                                                stream_of(x)),
+            "linear_cross_entropy forward");
+    } else if (a.reduction != DK_REDUCE_NONE) {
+      out.fill_(a.reduction == DK_REDUCE_MEAN ? std::numeric_limits<double>::quiet_NaN() : 0.0);
+    }
+  }
+  if (grad) {
+    auto node = std::make_shared<LinearCrossEntropyBackward>();
+    node->set_next_edges(collect_next_edges(input, weight, bias, target));
+    node->input = SavedVariable(x, false), node->weight = SavedVariable(w, false), node->target = SavedVariable(y, false);
+    node->has_bias = b.defined();
+    if (b.defined()) node->bias = SavedVariable(b, false);
+    node->saved = saved, node->a = a;
+    node->in_sizes = input.sizes().vec(), node->out_sizes = out.sizes().vec();
+    torch::autograd::set_history(out, node);
+  }
+  return out;
+}
+
 // ------------------------------------------------------------------ Python surface
 
 Tensor tensor_arg(PyObject* o, const char* name, bool optional = false) {
@@ -609,6 +790,21 @@ double double_arg(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw python_error();
   return v;
+}
+// any integer, modulo 2^64
+unsigned long long word_arg(PyObject* o) {
+  const unsigned long long v = PyLong_AsUnsignedLongLongMask(o);
+  if (v == (unsigned long long)-1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+int reduction_arg(PyObject* o) {
+  if (PyUnicode_Check(o)) {
+    if (!PyUnicode_CompareWithASCIIString(o, "mean")) return DK_REDUCE_MEAN;
+    if (!PyUnicode_CompareWithASCIIString(o, "sum")) return DK_REDUCE_SUM;
+    if (!PyUnicode_CompareWithASCIIString(o, "none")) return DK_REDUCE_NONE;
+  }
+  TORCH_CHECK_VALUE(false, "reduction must be 'none', 'mean' or 'sum'");
+  return 0;
 }
 ConvArgs conv_args(PyObject* const* a) {
   ConvArgs c;
@@ -673,6 +869,29 @@ DK_METHOD(py_clip_offsets, 6, {
   DK_NOGIL(clip_offsets(o, b, lo, hi, dilate, post));
 })
 
+// dropout(input, p, seed or [seed, offset] on the device, offset, shared_dims)
+DK_METHOD(py_dropout, 5, {
+  const Tensor x = tensor_arg(a[0], "input");
+  const double p = double_arg(a[1]);
+  Tensor state;
+  if (THPVariable_Check(a[2])) state = THPVariable_Unpack(a[2]);
+  const unsigned long long seed = state.defined() ? 0 : word_arg(a[2]), offset = word_arg(a[3]);
+  const int shared = int_arg(a[4]);
+  DK_NOGIL(dropout(x, p, state, seed, offset, shared));
+})
+DK_METHOD(py_linear_cross_entropy, 7, {
+  const Tensor x = tensor_arg(a[0], "input");
+  Tensor w = tensor_arg(a[1], "weight"), b = tensor_arg(a[3], "bias", true);
+  const Tensor y = tensor_arg(a[2], "target");
+  CrossEntropyArgs c;
+  c.ignore_index = PyLong_AsLongLong(a[4]);
+  if (c.ignore_index == -1 && PyErr_Occurred()) throw python_error();
+  c.reduction = reduction_arg(a[5]);
+  c.smoothing = double_arg(a[6]);
+  follow(w, x), follow(b, x);
+  DK_NOGIL(linear_cross_entropy(x, w, y, b, c));
+})
+
 // bind({name: address}, error class): the loaded library's entry points
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -711,6 +930,8 @@ PyMethodDef methods[] = {
     {"plane_scale", DK_FAST(py_plane_scale), METH_FASTCALL, nullptr},
     {"global_dk_scale", DK_FAST(py_global_dk_scale), METH_FASTCALL, nullptr},
     {"clip_offsets", DK_FAST(py_clip_offsets), METH_FASTCALL, nullptr},
+    {"dropout", DK_FAST(py_dropout), METH_FASTCALL, nullptr},
+    {"linear_cross_entropy", DK_FAST(py_linear_cross_entropy), METH_FASTCALL, nullptr},
     {"bind", DK_FAST(py_bind), METH_FASTCALL, nullptr},
     {"entry_points", py_entry_points, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -12,7 +12,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DK_B200_LIB", os.path.join(os.path.dirname(_HERE), "lib", "libdk_b200.so"))
 
-DK_F32, DK_F16, DK_F64 = 0, 1, 2
+DK_F32, DK_F16, DK_F64, DK_BF16 = 0, 1, 2, 3
 _DTYPES = {torch.float32: DK_F32, torch.float16: DK_F16, torch.float64: DK_F64}
 
 
@@ -69,6 +69,13 @@ _PROTOS = {
     "dk_global_dk_backward": (_int, [_vp] * 12 + [_int, _int, _int, _int, _ip, _int, _vp, ctypes.c_size_t, _vp]),
     "dk_offset_clip_forward": (_int, [_vp, _vp, _vp, _int, _int, _int] + [ctypes.c_double] * 4 + [_int, _vp]),
     "dk_offset_clip_backward": (_int, [_vp, _vp, _vp, _vp, _int, _int, _int] + [ctypes.c_double] * 4 + [_int, _vp]),
+    "dk_dropout": (_int, [_vp, _vp, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_double, ctypes.c_ulonglong,
+                          ctypes.c_ulonglong, _vp, _vp, _int, _vp]),
+    "dk_linear_cross_entropy_forward_workspace_bytes": (_sz, [_int] * 4),
+    "dk_linear_cross_entropy_forward": (_int, [_vp] * 6 + [_int] * 3 + [ctypes.c_longlong, _int, ctypes.c_double, _int, _vp, _sz, _vp]),
+    "dk_linear_cross_entropy_backward_workspace_bytes": (_sz, [_int] * 4),
+    "dk_linear_cross_entropy_backward": (_int, [_vp] * 9 + [_int] * 3 +
+                                         [ctypes.c_longlong, _int, ctypes.c_double, _int, _vp, _sz, _vp]),
     "dk_output_size": (_int, [_gp, _ip, _ip]),
     "dk_status_string": (ctypes.c_char_p, [_int]),
     "dk_last_cuda_error": (_int, []),

@@ -1,3 +1,4 @@
+from .classifier import Dropout, LinearCrossEntropy
 from .deform_conv import DeformConv2d
 from .deform_kernel import (
     GlobalDeformKernel2d,
@@ -12,4 +13,6 @@ __all__ = [
     'LocalDeformKernel2d',
     'DeformKernel2d',
     'DeformKernelConv2d',
+    'Dropout',
+    'LinearCrossEntropy',
 ]

@@ -42,7 +42,8 @@ typedef enum dk_status {
   DK_ERR_CUDA = 4             /* a CUDA runtime call or launch failed; see dk_last_cuda_error() */
 } dk_status;
 
-typedef enum dk_dtype { DK_F32 = 0, DK_F16 = 1, DK_F64 = 2 } dk_dtype;
+/* DK_BF16: the classifier head's entry points only (dk_dropout, dk_linear_cross_entropy_*) */
+typedef enum dk_dtype { DK_F32 = 0, DK_F16 = 1, DK_F64 = 2, DK_BF16 = 3 } dk_dtype;
 
 /* Devices and numeric limits.  Every pointer of a call must belong to the CURRENT device (cudaGetDevice()): the library
  * launches there, on the given stream, and never checks ownership.  fp16 calls on the tensor-core path (3x3, pad 1,
@@ -282,6 +283,39 @@ int dk_offset_clip_forward(const void *offsets, const void *bias, void *output, 
 int dk_offset_clip_backward(const void *grad_output, const void *offsets, const void *bias, void *grad_offsets, int batch,
                             int channels, int plane_size, double lo, double hi, double dilate, double post_scale, int dtype,
                             void *stream);
+
+/* ---------------------------------------------------------------- classifier head: dropout
+ * (no counterpart in the reference, whose classifiers end in stock modules)
+ *   output[i] = draw(i / run) >= round(p * 2^32) ? input[i] / (1 - p) : 0
+ * `run` consecutive elements share a draw (1: every element has its own; a plane; a sample).  The draws are those of
+ * Philox4x32-10 under (seed, offset): the mask is never stored, and the backward is the same call on the gradient.
+ * state: device, two 64-bit words (seed, offset) read by the kernel, so that a captured call draws anew when the caller
+ * advances them; `offset` is added to the second, `seed` is not looked at; NULL: the arguments alone.  used: device, two
+ * 64-bit words that receive the seed and offset of this call (what its backward passes as `state`, with offset 0), or
+ * NULL.  0 <= p <= 1.  Dropped elements are zero whatever the input holds. */
+int dk_dropout(const void *input, void *output, long long count, long long run, double p, unsigned long long seed,
+               unsigned long long offset, const void *state, void *used, int dtype, void *stream);
+
+/* ---------------------------------------------------------------- classifier head: linear layer + softmax cross entropy
+ * z = input [rows, features] weight [classes, features]^T + bias [classes] (or NULL), never stored;
+ *   loss_t = logsumexp(z_t) - (1 - label_smoothing) z_t[target_t] - label_smoothing * mean(z_t)
+ * target [rows], 64-bit; rows whose target is ignore_index have no loss and no gradient, whatever their input holds; a
+ * target outside [0, classes) gives NaN.  reduction: DK_REDUCE_MEAN divides by the number of rows that count (none: the
+ * loss is NaN, the gradients are zero).  loss: one value, or [rows] for DK_REDUCE_NONE; it, `saved` and grad_loss are
+ * float (double for DK_F64).  saved: rows + 2 values that the backward takes back, or NULL.  input and weight begin on
+ * 16 bytes.  Any gradient may be NULL. */
+typedef enum dk_reduction { DK_REDUCE_NONE = 0, DK_REDUCE_MEAN = 1, DK_REDUCE_SUM = 2 } dk_reduction;
+size_t dk_linear_cross_entropy_forward_workspace_bytes(int rows, int features, int classes, int dtype);
+int dk_linear_cross_entropy_forward(const void *input, const void *weight, const void *bias, const long long *target,
+                                    void *loss, void *saved, int rows, int features, int classes, long long ignore_index,
+                                    int reduction, double label_smoothing, int dtype, void *workspace,
+                                    size_t workspace_bytes, void *stream);
+size_t dk_linear_cross_entropy_backward_workspace_bytes(int rows, int features, int classes, int dtype);
+int dk_linear_cross_entropy_backward(const void *grad_loss, const void *input, const void *weight, const void *bias,
+                                     const long long *target, const void *saved, void *grad_input, void *grad_weight,
+                                     void *grad_bias, int rows, int features, int classes, long long ignore_index,
+                                     int reduction, double label_smoothing, int dtype, void *workspace,
+                                     size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

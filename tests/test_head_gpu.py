@@ -1,0 +1,388 @@
+"""The classifier head on the GPU: dropout bit by bit, the loss and its gradients within derived bounds."""
+import pytest
+import torch
+
+import head_oracle as H
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def functions():
+    from deformable_kernels.ops.deform_kernel import functions as f
+    return f
+
+
+# ------------------------------------------------------------------ dropout
+
+@pytest.mark.parametrize("dtype", list(H.DTYPES))
+@pytest.mark.parametrize("shape, shared", [((1,), 0), ((7,), 0), ((8,), 0), ((9, 3), 1), ((300, 1001), 0), ((5, 6, 7, 9), 2), ((5, 6, 7, 9), 3),
+                                           ((4, 3, 64, 64), 2), ((3, 5, 2), 1), ((2, 3), 2), ((), 0)])
+def test_dropout_is_its_definition(shape, shared, dtype):
+    torch.manual_seed(1)
+    x = torch.randn(shape).to(H.DTYPES[dtype])
+    dy = torch.randn(shape).to(H.DTYPES[dtype])
+    for p, seed, offset in ((0.2, 12345, 0), (0.5, 2 ** 63 + 17, 2 ** 40 + 3)):
+        xg = x.to(DEV).requires_grad_(True)
+        y = functions().dropout(xg, p, seed, offset, shared_dims=shared)
+        dx, = torch.autograd.grad(y, xg, dy.to(DEV))
+        assert y.dtype == x.dtype and y.shape == x.shape
+        assert torch.equal(y.detach().cpu(), H.dropout(x, p, seed, offset, shared))
+        assert torch.equal(dx.cpu(), H.dropout(dy, p, seed, offset, shared))
+
+
+def test_dropout_looks_at_the_lower_half_where_the_upper_is_the_thresholds():
+    n = 1 << 19
+    x = torch.ones(n, device=DEV)
+    for p in (0.3, 1e-6, 2.0 ** -16, 1 - 2.0 ** -16, 2.0 ** -32):
+        assert torch.equal(functions().dropout(x, p, 77, 5).cpu(), H.dropout(torch.ones(n), p, 77, 5))
+    assert torch.equal(functions().dropout(x, 0.0, 1), x)
+    assert not functions().dropout(x, 1.0, 1).any()
+
+
+def test_dropout_of_values_that_are_not_finite_is_zero_where_dropped():
+    x = torch.tensor([float("inf"), float("nan"), float("-inf"), 1.0] * 64)
+    keep = H.keep_mask(x.shape, 0.5, 3, 0)
+    for t in (x, x.half()):
+        y = functions().dropout(t.to(DEV), 0.5, 3).cpu()
+        assert (y[~keep] == 0).all()
+        assert torch.equal(y[keep].isnan(), t[keep].isnan()) and torch.equal(y[keep].isinf(), t[keep].isinf())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+def test_dropout_of_views(dtype):
+    base = torch.randn(6, 40, 33).to(H.DTYPES[dtype])
+    for view in (lambda t: t[:, 1:, 3:], lambda t: t.transpose(0, 2), lambda t: t.flatten()[1:], lambda t: t[:, :1].expand(6, 5, 33)):
+        y = functions().dropout(view(base.to(DEV)), 0.3, 4)
+        assert torch.equal(y.cpu(), H.dropout(view(base).contiguous(), 0.3, 4))
+
+
+def test_dropout_state_on_the_device_and_replayed_graphs():
+    x = torch.randn(1000, device=DEV)
+    state = torch.tensor([99, 10], device=DEV)
+    want = [H.dropout(x.cpu(), 0.4, 99, 10 + i) for i in range(6)]
+    assert torch.equal(functions().dropout(x, 0.4, state).cpu(), want[0])
+    assert torch.equal(functions().dropout(x, 0.4, state, 2).cpu(), want[2])
+    # the backward draws what its forward drew, although the state has moved on
+    xg = x.clone().requires_grad_(True)
+    y = functions().dropout(xg, 0.4, state)
+    state[1] += 1
+    dx, = torch.autograd.grad(y, xg, x)
+    assert torch.equal(y.detach().cpu(), want[0]) and torch.equal(dx.cpu(), want[0])
+
+    from deformable_kernels.modules import Dropout
+    m = Dropout(0.4, seed=99)
+    xs = x.clone().requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(m(xs), xs, x)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = m(xs)
+        dx, = torch.autograd.grad(y, xs, x)
+    m.set_rng_state([99, 10])
+    for i in range(3):
+        g.replay()
+        assert torch.equal(y.detach().cpu(), want[i]) and torch.equal(dx.cpu(), want[i])
+    assert m.rng_state() == [99, 13]
+
+
+def test_dropout_refusals():
+    f = functions()
+    x = torch.zeros(4, 4, device=DEV)
+    for kw in (dict(p=1.5), dict(p=-0.5), dict(p=float("nan")), dict(shared_dims=3), dict(shared_dims=-1),
+               dict(seed=torch.zeros(3, dtype=torch.int64, device=DEV))):
+        with pytest.raises(ValueError):
+            f.dropout(x, **kw)
+    with pytest.raises(TypeError):
+        f.dropout(x, 0.5, torch.zeros(2, device=DEV))
+    with pytest.raises(TypeError):
+        f.dropout(x.int(), 0.5, 1)
+    with pytest.raises(NotImplementedError):
+        f.dropout(x, 0.5, torch.zeros(2, dtype=torch.int64))
+    assert f.dropout(x[:0], 0.5, 1).shape == (0, 4)
+
+
+# ------------------------------------------------------------------ linear layer + cross entropy
+
+def make(t, d, v, dtype, bias=True, ignored=0.0, reduction="mean", seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    dt = H.DTYPES[dtype]
+    w = (torch.randn(v, d, generator=gen) * (1.5 / d ** 0.5)).to(dt)
+    y = torch.randint(0, v, (t,), generator=gen)
+    x = (torch.randn(t, d, generator=gen) + 3 * torch.rand(t, 1, generator=gen) * w[y].float()).to(dt)
+    b = (torch.randn(v, generator=gen) * 0.1).to(dt) if bias else None
+    if ignored:
+        y = torch.where(torch.rand(t, generator=gen) < ignored, torch.full_like(y, -100), y)
+    scale = 1024.0 if dtype == "fp16" else 1.0
+    up = torch.rand(t, generator=gen) * scale if reduction == "none" else torch.tensor(scale / (t if reduction == "sum" else 1))
+    return x, w, y, b, up.double() if dtype == "fp64" else up
+
+
+def check(x, w, y, b, up, where="", **kw):
+    """One call and its gradients against the 64-bit oracle, every value within its bound."""
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b) if t is not None]
+    loss = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), leaves[2] if b is not None else None, **kw)
+    grads = torch.autograd.grad(loss, leaves, up.to(DEV))
+    out, far = H.head(x, w, y, b, up, **kw)
+    got = dict(zip(("loss", "dx", "dw", "db"), (loss.detach(),) + grads))
+    assert loss.dtype == (torch.float64 if x.dtype == torch.float64 else torch.float32)
+    for name, v in got.items():
+        v = v.cpu()
+        assert v.dtype == (loss.dtype if name == "loss" else x.dtype) and v.shape == out[name].shape, name
+        assert torch.isfinite(v).all() == torch.isfinite(out[name]).all(), (where, name)
+        over = ((v.double() - out[name]).abs() / far[name]).nan_to_num(0).max().item() if v.numel() else 0
+        assert over <= 1, (where, name, over, (v.double() - out[name]).abs().max().item(), out[name].abs().max().item())
+    with torch.no_grad():
+        again = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), leaves[2] if b is not None else None, **kw)
+    assert torch.equal(again, loss.detach()) or not torch.isfinite(again).all()
+    return got
+
+
+SIZES = [(1, 8, 2), (1, 1280, 1000), (2, 1, 1), (31, 24, 7), (33, 33, 65), (127, 64, 130), (128, 128, 256), (129, 200, 257), (300, 96, 1000),
+         (257, 65, 1031), (64, 520, 4099), (1030, 40, 64)]
+
+
+@pytest.mark.parametrize("dtype", list(H.DTYPES))
+@pytest.mark.parametrize("t, d, v", SIZES)
+def test_head_sizes(t, d, v, dtype):
+    check(*make(t, d, v, dtype, seed=t + d + v))
+
+
+@pytest.mark.parametrize("dtype", list(H.DTYPES))
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1, 1.0])
+def test_head_options(dtype, reduction, smoothing):
+    for bias, ignored in ((True, 0.0), (False, 0.3)):
+        check(*make(150, 72, 203, dtype, bias, ignored, reduction, seed=5), reduction=reduction, label_smoothing=smoothing)
+
+
+@pytest.mark.parametrize("dtype", list(H.DTYPES))
+def test_ignored_rows_have_no_say_whatever_they_hold(dtype):
+    x, w, y, b, up = make(140, 48, 90, dtype, ignored=0.4, seed=6)
+    dead = y == -100
+    clean = check(x, w, y, b, up)
+    for bad in (float("nan"), float("inf"), float("-inf"), torch.finfo(x.dtype).max):
+        x2 = x.clone()
+        x2[dead] = bad
+        dirty = check(x2, w, y, b, up)
+        for k in clean:
+            assert torch.equal(clean[k], dirty[k]), (k, bad)
+    y2 = torch.where(dead, torch.full_like(y, 255), y)
+    other = check(x, w, y2, b, up, ignore_index=255)
+    assert all(torch.equal(clean[k], other[k]) for k in clean)
+
+
+@pytest.mark.parametrize("dtype", list(H.DTYPES))
+def test_all_rows_ignored(dtype):
+    x, w, y, b, up = make(40, 16, 10, dtype)
+    y[:] = -100
+    for reduction, want in (("mean", float("nan")), ("sum", 0.0), ("none", 0.0)):
+        u = up if reduction != "none" else up * torch.ones(40, dtype=up.dtype)
+        leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+        loss = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), leaves[2], reduction=reduction)
+        grads = torch.autograd.grad(loss, leaves, u.to(DEV))
+        assert torch.isnan(loss).all() if want != want else (loss == want).all()
+        assert all((g == 0).all() for g in grads)
+
+
+@pytest.mark.parametrize("dtype", list(H.DTYPES))
+def test_classes_taken_out_by_an_infinite_bias(dtype):
+    x, w, y, b, up = make(70, 40, 300, dtype, seed=8)
+    out = torch.rand(300, generator=torch.Generator().manual_seed(1)) < 0.5
+    out[y] = False
+    out[64:192] = True
+    y[y >= 64] = int((~out).nonzero()[0])
+    b[out] = float("-inf")
+    b[y] = 0.0
+    check(x, w, y, b, up)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+def test_targets_that_are_no_class_make_the_loss_nan(dtype):
+    x, w, y, b, up = make(130, 40, 30, dtype, reduction="none")
+    for wrong in (30, -1, 2 ** 40, -(2 ** 62)):
+        y2 = y.clone()
+        y2[7] = wrong
+        leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+        loss = functions().linear_cross_entropy(leaves[0], leaves[1], y2.to(DEV), leaves[2], reduction="none")
+        dx, dw, db = torch.autograd.grad(loss, leaves, up.to(DEV))
+        bad = torch.isnan(loss)
+        assert bad[7] and int(bad.sum()) == 1
+        assert torch.isnan(dx[7]).all() and torch.isfinite(dx[8:]).all() and torch.isfinite(dx[:7]).all()
+        assert torch.isnan(dw).all() and torch.isnan(db).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_rows_with_features_that_are_not_finite_keep_to_themselves(dtype):
+    x, w, y, b, up = make(130, 40, 300, dtype, reduction="none")
+    x[5, 3], x[77, 0] = float("nan"), float("inf")
+    loss = functions().linear_cross_entropy(x.to(DEV), w.to(DEV), y.to(DEV), b.to(DEV), reduction="none").cpu()
+    bad = torch.isnan(loss)
+    assert bad[5] and bad[77] and int(bad.sum()) == 2
+
+
+def test_large_and_small_logits():
+    """Logits of a few hundred: the sum of exponentials is taken from the largest one."""
+    for dtype in H.DTYPES:
+        x, w, y, b, up = make(50, 64, 200, dtype, seed=3)
+        check(x * 16, w * 4, y, b, up)
+        check(x * 0, w, y, b, up)
+
+
+def test_leading_dimensions_views_and_dtypes():
+    f = functions()
+    x, w, y, b, up = make(60, 32, 50, "fp16", seed=4)
+    base = check(x, w, y, b, up)
+    # [N, H, W, features] and a transposed feature map
+    x4 = x.view(3, 4, 5, 32).to(DEV).requires_grad_(True)
+    loss = f.linear_cross_entropy(x4, w.to(DEV), y.view(3, 4, 5).to(DEV), b.to(DEV))
+    dx, = torch.autograd.grad(loss, x4, up.to(DEV))
+    assert torch.equal(loss.detach(), base["loss"]) and torch.equal(dx.view(60, 32), base["dx"])
+    xt = x.t().contiguous().to(DEV).requires_grad_(True)
+    loss = f.linear_cross_entropy(xt.t(), w.to(DEV), y.to(DEV), b.to(DEV))
+    dxt, = torch.autograd.grad(loss, xt, up.to(DEV))
+    assert torch.equal(loss.detach(), base["loss"]) and torch.equal(dxt.t(), base["dx"])
+    assert torch.equal(f.linear_cross_entropy(x4.detach(), w.to(DEV), y.view(3, 4, 5).to(DEV), b.to(DEV), reduction="none").view(60),
+                       f.linear_cross_entropy(x.to(DEV), w.to(DEV), y.to(DEV), b.to(DEV), reduction="none"))
+    # storage that does not begin on 16 bytes, a strided target
+    odd = torch.cat([x.flatten()[:1], x.flatten()]).to(DEV)[1:].view(60, 32)
+    oddw = torch.cat([w.flatten()[:3], w.flatten()]).to(DEV)[3:].view(50, 32)
+    y2 = torch.stack([y, y], 1).to(DEV)[:, 0]
+    assert torch.equal(f.linear_cross_entropy(odd, oddw, y2, b.to(DEV)), base["loss"])
+    # fp32 parameters follow 16-bit features, and get fp32 gradients
+    wp, bp = w.float().to(DEV).requires_grad_(True), b.float().to(DEV).requires_grad_(True)
+    loss = f.linear_cross_entropy(x.to(DEV), wp, y.to(DEV), bp)
+    dw, db = torch.autograd.grad(loss, [wp, bp], up.to(DEV))
+    assert dw.dtype == db.dtype == torch.float32
+    assert torch.equal(dw.half(), base["dw"]) and torch.equal(db.half(), base["db"])
+
+
+def test_single_gradients_and_empty_batches():
+    f = functions()
+    x, w, y, b, up = (t.to(DEV) for t in make(60, 32, 50, "fp32", seed=4))
+    full = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(f.linear_cross_entropy(full[0], full[1], y, full[2]), full, up)
+    for i in range(3):
+        part = [x, w, b]
+        part[i] = part[i].clone().requires_grad_(True)
+        got, = torch.autograd.grad(f.linear_cross_entropy(part[0], part[1], y, part[2]), part[i], up)
+        assert torch.equal(got, want[i])
+    for reduction in ("none", "mean", "sum"):
+        leaves = [x[:0].clone().requires_grad_(True), w.clone().requires_grad_(True), b.clone().requires_grad_(True)]
+        loss = f.linear_cross_entropy(leaves[0], leaves[1], y[:0], leaves[2], reduction=reduction)
+        assert {"none": loss.shape == (0,), "mean": loss.isnan().all(), "sum": (loss == 0).all()}[reduction]
+        dx, dw, db = torch.autograd.grad(loss.sum(), leaves)
+        assert dx.shape == (0, 32) and (dw == 0).all() and (db == 0).all()
+
+
+def test_refusals():
+    f = functions()
+    x, w, y, b, _ = (t.to(DEV) for t in make(6, 8, 5, "fp32"))
+    for args in ((x, w[:, :7], y), (x, w, y[:5]), (x, w.flatten(), y), (x, w, y.view(6, 1)), (x, w, y, b[:4]), (x, w[:0], y), (x[:, :0], w[:, :0], y)):
+        with pytest.raises(ValueError):
+            f.linear_cross_entropy(*args)
+    for kw in (dict(label_smoothing=1.1), dict(label_smoothing=-0.1), dict(reduction="max")):
+        with pytest.raises(ValueError):
+            f.linear_cross_entropy(x, w, y, b, **kw)
+    for args in ((x, w, y.int()), (x, w, y.float()), (x.int(), w.int(), y)):
+        with pytest.raises(TypeError):
+            f.linear_cross_entropy(*args)
+    with pytest.raises(NotImplementedError):
+        f.linear_cross_entropy(x, w, y.cpu())
+    loss = f.linear_cross_entropy(x.requires_grad_(True), w, y)
+    loss.backward()
+    with pytest.raises(RuntimeError):
+        loss.backward()
+    loss = f.linear_cross_entropy(x, w, y)
+    with torch.no_grad():
+        x += 1
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+
+def test_gradients_against_differences():
+    """fp64, central differences of the operator itself: the step 1e-5 leaves h^2 / 6 of a third derivative that is
+    below one, and 2^-52 / h of a loss below ten: under 1e-8 together."""
+    x, w, y, b, _ = make(9, 6, 5, "fp64", ignored=0.2, seed=12)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    for kw in (dict(), dict(label_smoothing=0.2, reduction="sum")):
+        grads = torch.autograd.grad(functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), leaves[2], **kw), leaves)
+        for i, g in enumerate(grads):
+            for j in range(0, g.numel(), 3):
+                at = []
+                for s in (1e-5, -1e-5):
+                    moved = [t.detach().clone() for t in leaves]
+                    moved[i].view(-1)[j] += s
+                    at.append(functions().linear_cross_entropy(moved[0], moved[1], y.to(DEV), moved[2], **kw).item())
+                assert abs((at[0] - at[1]) / 2e-5 - g.view(-1)[j].item()) < 1e-8
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_the_same_call_gives_the_same_bits(dtype):
+    args = make(700, 136, 1500, dtype, ignored=0.1, seed=9)
+    a, b = check(*args), check(*args)
+    assert all(torch.equal(a[k], b[k]) for k in a)
+
+
+def test_head_on_another_stream_and_captured():
+    f = functions()
+    x, w, y, b, up = (t.to(DEV) for t in make(200, 64, 500, "bf16", seed=2))
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+    def step():
+        loss = f.linear_cross_entropy(x, w, y, b, label_smoothing=0.1)
+        return (loss.detach(),) + torch.autograd.grad(loss, leaves, up)
+    want = [t.clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [t.clone() for t in step()]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, c) for a, c in zip(want, got))
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    for _ in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn_like(x))
+        want = [t.clone() for t in step()]
+        for g, out in graphs:
+            g.replay()
+        for g, out in graphs:
+            assert all(torch.equal(a, c) for a, c in zip(want, out))
+
+
+def test_head_and_dropout_together_as_a_training_step():
+    """Features -> dropout -> linear -> loss, as the module runs it, against the oracles one after the other."""
+    from deformable_kernels.modules import LinearCrossEntropy
+    torch.manual_seed(5)
+    x, w, y, b, up = make(90, 56, 120, "fp32", seed=15)
+    head = LinearCrossEntropy(56, 120, dropout=0.25, label_smoothing=0.1).to(DEV)
+    head.dropout.set_rng_state([41, 3])
+    with torch.no_grad():
+        head.weight.copy_(w), head.bias.copy_(b)
+    for step in range(3):
+        xg = x.to(DEV).requires_grad_(True)
+        loss = head(xg, y.to(DEV))
+        dx, dw, db = torch.autograd.grad(loss, [xg, head.weight, head.bias])
+        dropped = H.dropout(x, 0.25, 41, 3 + step)
+        out, far = H.head(dropped, w, y, b, torch.tensor(1.0), label_smoothing=0.1)
+        keep = H.keep_mask(x.shape, 0.25, 41, 3 + step).double() / 0.75
+        out["dx"], far["dx"] = out["dx"] * keep, far["dx"] * keep + out["dx"].abs() * 2.0 ** -22 + 1e-300
+        for name, v in (("loss", loss), ("dx", dx), ("dw", dw), ("db", db)):
+            assert ((v.detach().cpu().double() - out[name]).abs() <= far[name]).all(), (step, name)
+    head.eval()
+    with torch.no_grad():
+        assert torch.equal(head(x.to(DEV), y.to(DEV)), functions().linear_cross_entropy(x.to(DEV), head.weight, y.to(DEV), head.bias,
+                                                                                       label_smoothing=0.1))
+    with torch.autocast("cuda", dtype=torch.float16):
+        loss = head(x.to(DEV), y.to(DEV))
+        assert loss.dtype == torch.float32
+        loss.backward()
+    assert head.weight.grad.dtype == torch.float32
