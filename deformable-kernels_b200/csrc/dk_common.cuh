@@ -227,6 +227,9 @@ double local_conv_mma_items(const Geom& g, bool transposed);  // of 8 pixels and
 bool local_conv_mma_small(const Geom& g, bool transposed);  // and the call is so small that its block shape makes it the fastest one
 bool local_conv_mma_takes(const Geom& g, bool transposed);  // the band kernels have a block shape for this call
 int tc_error_status();
+namespace head {
+int head_error_status();
+}
 int tc_register_query(long long out[8]);  // {kernels, fewest registers per thread of any, what the roles' shares need}
 // gradients towards offsets and bank in fp32 arithmetic (dk_local_f32.cu); the bank's leave as *blocks partial sums [block][C][cells]
 template <typename T>

@@ -1,0 +1,996 @@
+// The three products of the classifier head on the fifth-generation tensor cores: logits with the statistics of their rows
+// (forward), logits with dz (backward), and both gradient products in one launch.
+//
+// One persistent kernel with one block per SM; where there are enough tiles two SMs share one of 256 x 256
+// (cta_group::2: each holds 128 rows of either operand in shared memory and 128 rows of the accumulator in TMEM), else
+// each has its own of 128 x BN.  Warp 0 fills a ring of shared-memory stages by TMA, warp 1 of the leading block issues
+// the mma, the last eight warps take the finished accumulator out of TMEM while the other half of TMEM receives the next
+// tile.  An operand is K-major (rows of the tensor are rows of the product) or MN-major (columns are); both
+// come as boxes of 64 x 64 values, 128 swizzled bytes a row.
+//
+// fp32 operands are three bf16 pieces each (8 bits a piece, 24 in all); the six products of pieces that reach 2^-24 are summed
+// in the same accumulator, the smallest first, so that the additions that cut are those of small sums.
+#include <math_constants.h>
+
+#include <type_traits>
+
+#include "dk_head.cuh"
+#include "dk_tc.cuh"
+
+namespace dk {
+namespace head {
+
+using ring::smem_u32;
+
+namespace {
+
+__device__ int g_head_error;  // set when a bounded wait ran out
+
+constexpr int kBox = 64;                    // values per side of a TMA box
+constexpr int kBoxBytes = kBox * kBox * 2;  // 8192
+constexpr int kStages = 6;
+constexpr int kThreads = 384;
+constexpr int kStageWarp = 4096;            // staging of an epilogue warp: 32 rows of 128 bytes
+
+struct SharedTail {
+  float bias[2][256];
+  unsigned long long full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+  unsigned tmem;
+  int abort_flag;
+};
+
+template <int CG, int BN>
+__host__ __device__ constexpr int stage_bytes() { return 128 * 128 + BN / CG * 128; }
+template <int CG, int BN>
+constexpr int smem_bytes() { return kStages * stage_bytes<CG, BN>() + 8 * kStageWarp + (int)sizeof(SharedTail); }
+
+// ---- PTX
+
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// the address of the same variable in block `rank` of the cluster
+__device__ __forceinline__ unsigned map_rank(unsigned addr, unsigned rank) {
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(unsigned bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(unsigned slot) {
+  if (CG == 1) {
+    tc::tmem_alloc_all(slot);
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free(unsigned addr) {
+  if (CG == 1) tc::tmem_free_all(addr);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;\n" ::"r"(addr) : "memory");
+}
+// all mma of this thread so far -> one arrival on `bar`, in both blocks of a pair
+template <int CG>
+__device__ __forceinline__ void commit(unsigned bar) {
+  if (CG == 1) {
+    tc::commit(bar);
+  } else {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar),
+                 "h"((unsigned short)3)
+                 : "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void mma_ss(unsigned d, uint64_t a, uint64_t b, unsigned idesc, bool acc) {
+  if (CG == 1)
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"((unsigned)acc)
+                 : "memory");
+  else
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"((unsigned)acc)
+                 : "memory");
+}
+// One box into this block's shared memory; a pair counts the bytes of both blocks on the leader's barrier.
+template <int CG>
+__device__ __forceinline__ void load_box(unsigned dst, const CUtensorMap* tm, int x, int y, int z, unsigned bar) {
+  if (CG == 1)
+    ring::tma_load_3d(dst, tm, x, y, z, bar);
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+            dst),
+        "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void store_box(const CUtensorMap* tm, unsigned src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];\n" ::"l"(tm), "r"(x), "r"(y), "r"(z),
+               "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+}
+__device__ __forceinline__ void stores_have_read() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
+
+__device__ __forceinline__ void ld32(float (&r)[32], unsigned a) {
+  unsigned* u = reinterpret_cast<unsigned*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+        "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]),
+        "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
+        "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(a));
+}
+__device__ __forceinline__ void wait_ld(float (&r)[32]) {
+  unsigned* u = reinterpret_cast<unsigned*>(r);
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]), "+r"(u[8]), "+r"(u[9]),
+                 "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15]), "+r"(u[16]), "+r"(u[17]), "+r"(u[18]),
+                 "+r"(u[19]), "+r"(u[20]), "+r"(u[21]), "+r"(u[22]), "+r"(u[23]), "+r"(u[24]), "+r"(u[25]), "+r"(u[26]), "+r"(u[27]),
+                 "+r"(u[28]), "+r"(u[29]), "+r"(u[30]), "+r"(u[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// ---- descriptors
+template <typename E>
+__host__ __device__ constexpr unsigned type_bits() { return sizeof(E) == 2 && std::is_same<E, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u; }
+// operand of 128-byte rows, swizzled in groups of eight rows.  K-major: `lead` is not looked at, `stride` = bytes between groups of eight
+// rows; MN-major: `lead` = bytes between blocks of 64 columns, `stride` = between groups of eight rows (of K)
+__device__ __forceinline__ uint64_t swizzled(unsigned addr, unsigned lead, unsigned stride) {
+  return tc::sdesc(addr, lead, stride) | (2ull << 61);
+}
+
+// ---- a wait of a whole warp that ends: true once any thread of the block gave up
+__device__ __forceinline__ bool try_wait(unsigned bar, unsigned parity) {
+  unsigned ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait(unsigned bar, unsigned parity, volatile int* abort_flag) {
+  bool done = try_wait(bar, parity);
+  for (unsigned i = 0; !done && i < ring::kMaxPolls && !*abort_flag; ++i) done = try_wait(bar, parity);
+  if (!done) *abort_flag = 1;
+  return __any_sync(0xffffffffu, *abort_flag != 0);
+}
+
+// 16-byte piece q of row r in a staging buffer of 128-byte rows
+__device__ __forceinline__ unsigned staged(unsigned base, int r, int q) { return base + r * 128 + ((q ^ (r & 7)) << 4); }
+__device__ __forceinline__ void sts16(unsigned a, unsigned x, unsigned y, unsigned z, unsigned w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(unsigned a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned lds4(unsigned a) {
+  unsigned v;
+  asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+template <typename E> __device__ __forceinline__ unsigned pack(float a, float b);
+template <> __device__ __forceinline__ unsigned pack<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+template <> __device__ __forceinline__ unsigned pack<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+template <typename E> __device__ __forceinline__ float2 unpack(unsigned v);
+template <> __device__ __forceinline__ float2 unpack<__half>(unsigned v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(unsigned v) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+
+// ---- arguments
+
+enum Role { kStats, kDz, kGrad };
+
+// one of the gradient products, out[M][N] = sum over K; tiles [splits][m][n]
+struct Product {
+  int M, N, blocks;           // blocks: 64-deep steps of K
+  int tiles_m, tiles_n, splits, per;  // per: steps of a split
+  float* acc;                 // running sum over the pieces, or [splits][M][N]
+  void* out;                  // NULL: the sums stay in acc
+  int first;                  // 0: add what acc holds
+};
+
+struct Args {
+  CUtensorMap x, x_clean, w, dz, dz_out;
+  // logits
+  int rows, classes;          // of this piece
+  int row0, class0;           // where the piece begins
+  int depth;                  // 64-deep steps over the features
+  int tiles_m, tiles_n, group;
+  const void* bias;           // of the parameters' type, or NULL
+  const long long* target;    // of the piece's first row
+  long long ignore;
+  float* top;                 // [slots][rows]
+  float* sum;
+  float* all;                 // NULL without label smoothing
+  float* picked;
+  const float* lse2;
+  const float* g;
+  float* column_sums;         // [rows / 32][classes], NULL: no bias gradient
+  float smooth_each, smooth_own;  // s / V, 1 - s
+  // gradients
+  Product dw, dx;
+  const float* strange;       // != 0: some ignored row's features are not finite, x_clean has them zeroed
+  const float* back;          // what the gradients are multiplied with (fp16: dz is scaled); NULL: nothing
+};
+
+struct Item {
+  int product;  // gradients: 0 dw, 1 dx
+  int m, n;     // tile
+  int split, first, count;  // steps of K
+};
+
+template <int ROLE>
+__device__ __forceinline__ int items_of(const Args& a) {
+  if (ROLE != kGrad) return a.tiles_m * a.tiles_n;
+  return a.dw.tiles_m * a.dw.tiles_n * a.dw.splits + a.dx.tiles_m * a.dx.tiles_n * a.dx.splits;
+}
+template <int ROLE>
+__device__ __forceinline__ Item item_of(const Args& a, int i) {
+  Item t;
+  t.product = 0, t.split = 0, t.first = 0, t.count = a.depth;
+  if (ROLE != kGrad) {
+    // columns of tiles, `group` tiles of rows high: their part of x stays in L2 while the weights stream past once a group
+    const int per = a.group * a.tiles_n, gi = i / per, left = a.tiles_m - gi * a.group, high = left < a.group ? left : a.group;
+    const int r = i - gi * per;
+    t.n = r / high, t.m = gi * a.group + r - t.n * high;
+    return t;
+  }
+  const int own = a.dw.tiles_m * a.dw.tiles_n * a.dw.splits;
+  t.product = i >= own;
+  const Product& p = t.product ? a.dx : a.dw;
+  if (t.product) i -= own;
+  t.n = i % p.tiles_n, i /= p.tiles_n;
+  t.m = i % p.tiles_m, t.split = i / p.tiles_m;
+  t.first = t.split * p.per;
+  t.count = p.blocks - t.first < p.per ? p.blocks - t.first : p.per;
+  return t;
+}
+
+// ---- the kernel
+
+template <int CG, int BN, int ROLE, typename E, int PIECES>
+__global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant__ Args a) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  constexpr int kStage = stage_bytes<CG, BN>();
+  constexpr int kBoxesB = BN / CG / kBox;          // boxes of B a block loads
+  constexpr int kGroups = BN >= 128 ? 2 : 1;       // epilogue warps side by side
+  constexpr int kWide = BN / kGroups;              // columns of an epilogue warp
+  constexpr int kPairs = PIECES == 1 ? 1 : 6;
+  SharedTail& t = *reinterpret_cast<SharedTail*>(smem + kStages * kStage + 8 * kStageWarp);
+  const unsigned base = smem_u32(smem);
+  if (base & 1023) {  // the swizzled boxes need it; the same in every block
+    if (threadIdx.x == 0) g_head_error = 2;
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned rank = CG == 1 ? 0u : cluster_rank();
+  const int cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
+  const int items = items_of<ROLE>(a);
+  volatile int* abort_flag = &t.abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) ring::mbar_init(smem_u32(&t.full[s]), 1), ring::mbar_init(smem_u32(&t.empty[s]), 1);
+    for (int b = 0; b < 2; ++b) ring::mbar_init(smem_u32(&t.acc_full[b]), 1), ring::mbar_init(smem_u32(&t.acc_empty[b]), CG * 4 * kGroups);
+    t.abort_flag = 0;
+    ring::fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc<CG>(smem_u32(&t.tmem));
+  tc::fence_before();
+  if (CG == 1) __syncthreads();
+  else cluster_sync();
+  tc::fence_after();
+  const unsigned tmem = t.tmem;
+
+  if (warp == 0) {
+    // ---------------- producer
+    const bool one = tc::elect_one();
+    const CUtensorMap* mx = &a.x;
+    if (ROLE == kGrad && a.strange && *a.strange != 0.0f) mx = &a.x_clean;
+    int fill = 0;
+    for (int i = cluster; i < items; i += clusters) {
+      const Item it = item_of<ROLE>(a, i);
+      const int m0 = (it.m * CG + (int)rank) * 128, n0 = it.n * BN + (int)rank * (BN / CG);
+      for (int pr = 0; pr < kPairs; ++pr) {
+        // smallest first: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+        const int pa = PIECES == 1 ? 0 : (0x001012 >> (4 * pr)) & 15, pb = PIECES == 1 ? 0 : (0x010210 >> (4 * pr)) & 15;
+        for (int kb = it.first; kb < it.first + it.count; ++kb, ++fill) {
+          const int s = fill % kStages;
+          if (wait(smem_u32(&t.empty[s]), ((fill / kStages) & 1) ^ 1, abort_flag)) continue;
+          const unsigned sa = base + s * kStage, sb = sa + 128 * 128;
+          unsigned bar = smem_u32(&t.full[s]);
+          if (CG == 2) bar = map_rank(bar, 0);
+          if (one) {
+            if (rank == 0) ring::mbar_arrive_expect_tx(smem_u32(&t.full[s]), CG * kStage);
+            const int k0 = kb * kBox;
+            if (ROLE != kGrad) {
+              for (int q = 0; q < 2; ++q) load_box<CG>(sa + q * kBoxBytes, &a.x, k0, a.row0 + m0 + q * kBox, pa, bar);
+              for (int q = 0; q < kBoxesB; ++q) load_box<CG>(sb + q * kBoxBytes, &a.w, k0, a.class0 + n0 + q * kBox, pb, bar);
+            } else if (it.product == 0) {
+              for (int q = 0; q < 2; ++q) load_box<CG>(sa + q * kBoxBytes, &a.dz, m0 + q * kBox, k0, pa, bar);
+              for (int q = 0; q < kBoxesB; ++q) load_box<CG>(sb + q * kBoxBytes, mx, n0 + q * kBox, a.row0 + k0, pb, bar);
+            } else {
+              for (int q = 0; q < 2; ++q) load_box<CG>(sa + q * kBoxBytes, &a.dz, k0, m0 + q * kBox, pa, bar);
+              for (int q = 0; q < kBoxesB; ++q) load_box<CG>(sb + q * kBoxBytes, &a.w, n0 + q * kBox, a.class0 + k0, pb, bar);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    // every stage handed back: nothing of this block is in flight any more
+    for (int s = 0; s < kStages && s < fill; ++s) {
+      const int last = (fill - 1 - s) / kStages * kStages + s;
+      (void)wait(smem_u32(&t.empty[s]), (last / kStages) & 1, abort_flag);
+    }
+  } else if (warp == 1) {
+    // ---------------- mma, the leading block only
+    if (rank == 0) {
+      const bool one = tc::elect_one();
+      constexpr unsigned kDesc = (1u << 4) | type_bits<E>() | ((unsigned)(BN >> 3) << 17) | ((unsigned)(128 * CG >> 4) << 24);
+      int fill = 0, tile = 0;
+      for (int i = cluster; i < items; i += clusters, ++tile) {
+        const Item it = item_of<ROLE>(a, i);
+        // both operands of the logits are K-major; W and x of the gradients are MN-major, dz is either
+        const bool ta = ROLE == kGrad && it.product == 0, tb = ROLE == kGrad;
+        const unsigned idesc = kDesc | ((unsigned)ta << 15) | ((unsigned)tb << 16);
+        const unsigned lead = kBoxBytes, step_a = ta ? 2048 : 32, step_b = tb ? 2048 : 32;
+        const int b = tile & 1;
+        bool gone = wait(smem_u32(&t.acc_empty[b]), ((tile >> 1) & 1) ^ 1, abort_flag);
+        tc::fence_after();
+        const unsigned d = tmem + b * BN;
+        const int steps = it.count * kPairs;
+        for (int k = 0; k < steps; ++k, ++fill) {
+          const int s = fill % kStages;
+          gone = wait(smem_u32(&t.full[s]), (fill / kStages) & 1, abort_flag);
+          if (gone) continue;
+          tc::fence_after();
+          const unsigned sa = base + s * kStage, sb = sa + 128 * 128;
+          const uint64_t da = swizzled(sa, lead, 1024), db = swizzled(sb, lead, 1024);
+          if (one) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mma_ss<CG>(d, da + (uint64_t)(q * step_a >> 4), db + (uint64_t)(q * step_b >> 4), idesc, k > 0 || q > 0);
+            commit<CG>(smem_u32(&t.empty[s]));
+          }
+          __syncwarp();
+        }
+        if (one && !gone) commit<CG>(smem_u32(&t.acc_full[b]));
+        __syncwarp();
+      }
+    }
+  } else if (warp >= 4 && (warp - 4) >> 2 < kGroups) {
+    // ---------------- epilogue
+    const int sub = warp & 3, grp = (warp - 4) >> 2;
+    const unsigned stage = base + kStages * kStage + (warp - 4) * kStageWarp;
+    const unsigned lanes = (unsigned)(32 * sub) << 16;
+    constexpr float kL2 = (float)kLog2e;
+    int tile = 0;
+    for (int i = cluster; i < items; i += clusters, ++tile) {
+      const Item it = item_of<ROLE>(a, i);
+      const int b = tile & 1;
+      const int row_base = (it.m * CG + (int)rank) * 128 + 32 * sub, row = row_base + lane;
+      const int col_base = it.n * BN + grp * kWide;
+      float* bias = t.bias[b];
+      long long y = -1;
+      float l2 = 0, g = 0;
+      bool live = false;
+      if (ROLE != kGrad) {
+        // what is added to the logits; -inf outside, where the product is zero
+        for (int c = threadIdx.x - 128; c < BN; c += 128 * kGroups) {
+          const int v = it.n * BN + c;
+          bias[c] = v < a.classes ? (a.bias ? (PIECES == 1 ? (float)((const E*)a.bias)[a.class0 + v] : ((const float*)a.bias)[a.class0 + v]) : 0.0f)
+                                  : -CUDART_INF_F;
+        }
+        if (row < a.rows) {
+          y = a.target[row];
+          if (ROLE == kDz) l2 = a.lse2[row], g = a.g[row], live = y != a.ignore;
+        }
+        __syncwarp();
+        asm volatile("bar.sync 1, %0;\n" ::"n"(128 * kGroups) : "memory");
+      }
+      // the row's own class as a column of this warp, -1: elsewhere
+      const long long far = y - a.class0 - col_base;
+      const int own = far >= 0 && far < kWide ? (int)far : -1;
+      (void)wait(smem_u32(&t.acc_full[b]), (tile >> 1) & 1, abort_flag);
+      tc::fence_after();
+      const unsigned d = tmem + lanes + b * BN + grp * kWide;
+      if (ROLE == kStats) {
+        float top = -CUDART_INF_F, sum = 0, all = 0, picked = 0;
+#pragma unroll 1
+        for (int c0 = 0; c0 < kWide; c0 += 32) {
+          float z[32];
+          __syncwarp();
+          ld32(z, d + c0);
+          wait_ld(z);
+          const float4* bp = reinterpret_cast<const float4*>(bias + grp * kWide + c0);
+          float most = -CUDART_INF_F;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const float4 v = bp[q];
+            z[4 * q] += v.x, z[4 * q + 1] += v.y, z[4 * q + 2] += v.z, z[4 * q + 3] += v.w;
+          }
+          if (own >= c0 && own < c0 + 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (own == c0 + j) picked = z[j];
+          }
+          if (a.all) {
+            const int in = a.classes - col_base - c0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) all += j < in ? z[j] : 0.0f;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) most = fmaxf(most, z[j]);
+          const float n = fmaxf(top, most * kL2), ref = n == -CUDART_INF_F ? 0.0f : n;
+          float part = 0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) part += ex2(fmaf(z[j], kL2, -ref));
+          sum = sum * ex2(top - ref) + part;
+          top = n;
+        }
+        if (row < a.rows) {
+          const long long at = (long long)(it.n * kGroups + grp) * a.rows + row;
+          a.top[at] = top, a.sum[at] = sum;
+          if (a.all) a.all[at] = all;
+          if (own >= 0 && own + col_base < a.classes) a.picked[row] = picked;
+        }
+      } else if (ROLE == kDz) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < kWide; c0 += kBox) {
+          const bool inside = row_base < a.rows && col_base + c0 < a.classes;
+          if (!inside) break;  // of the whole warp
+          float v[2][32];
+          __syncwarp();
+          ld32(v[0], d + c0);
+          ld32(v[1], d + c0 + 32);
+          wait_ld(v[0]);
+          wait_ld(v[1]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4* bp = reinterpret_cast<const float4*>(bias + grp * kWide + c0 + 32 * h);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const float4 bb = bp[q];
+              v[h][4 * q] += bb.x, v[h][4 * q + 1] += bb.y, v[h][4 * q + 2] += bb.z, v[h][4 * q + 3] += bb.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              float p = ex2(fmaf(v[h][j], kL2, -l2)) - a.smooth_each;
+              if (own == c0 + 32 * h + j) p -= a.smooth_own;
+              v[h][j] = live ? p * g : 0.0f;
+            }
+          }
+          float s0 = 0, s1 = 0;
+#pragma unroll
+          for (int pc = 0; pc < PIECES; ++pc) {
+            if (lane == 0) stores_have_read();
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              unsigned w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float& v0 = v[q >> 2][(q & 3) * 8 + 2 * e];
+                float& v1 = v[q >> 2][(q & 3) * 8 + 2 * e + 1];
+                w[e] = pack<E>(v0, v1);
+                if (PIECES > 1) {
+                  const float2 f = unpack<E>(w[e]);
+                  v0 -= f.x, v1 -= f.y;
+                }
+              }
+              sts16(staged(stage, lane, q), w[0], w[1], w[2], w[3]);
+            }
+            ring::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) store_box(&a.dz_out, stage, col_base + c0, row_base, pc);
+            if (a.column_sums) {
+              // two columns a lane
+#pragma unroll 8
+              for (int r = 0; r < 32; ++r) {
+                const float2 f = unpack<E>(lds4(staged(stage, r, lane >> 2) + (lane & 3) * 4));
+                s0 += f.x, s1 += f.y;
+              }
+            }
+          }
+          if (a.column_sums) {
+            const int c = col_base + c0 + 2 * lane;
+            float* to = a.column_sums + (long long)(row_base >> 5) * a.classes + c;
+            if (c < a.classes) to[0] = s0;
+            if (c + 1 < a.classes) to[1] = s1;
+          }
+        }
+      } else {
+        const Product& p = it.product ? a.dx : a.dw;
+        const float back = a.back ? *a.back : 1.0f;
+        float* acc = p.acc ? p.acc + (p.splits > 1 ? (long long)it.split * p.M * p.N : 0) : nullptr;
+        const bool out16 = PIECES == 1 && p.out;  // 16-bit results; else fp32, to the gradient or to the sums
+        float* to32 = p.out ? (float*)p.out : acc;
+        const bool vec = (p.N & (out16 ? 7 : 3)) == 0;
+#pragma unroll 1
+        for (int c0 = 0; c0 < kWide; c0 += 32) {
+          if (row_base >= p.M || col_base + c0 >= p.N) break;  // of the whole warp
+          float v[32];
+          __syncwarp();
+          ld32(v, d + c0);
+          wait_ld(v);
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            sts16(staged(stage, lane, q), __float_as_uint(v[4 * q] * back), __float_as_uint(v[4 * q + 1] * back),
+                  __float_as_uint(v[4 * q + 2] * back), __float_as_uint(v[4 * q + 3] * back));
+          __syncwarp();
+          if (vec) {
+            // eight lanes a row: four values each
+#pragma unroll
+            for (int r4 = 0; r4 < 32; r4 += 4) {
+              const int r = r4 + (lane >> 3), q = lane & 7, c = col_base + c0 + 4 * q;
+              if (row_base + r < p.M && c < p.N) {
+                const uint4 u = lds16(staged(stage, r, q));
+                float4 f = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+                const long long at = (long long)(row_base + r) * p.N + c;
+                if (!p.first) {
+                  const float4 o = *reinterpret_cast<const float4*>(acc + at);
+                  f.x += o.x, f.y += o.y, f.z += o.z, f.w += o.w;
+                }
+                if (out16) *reinterpret_cast<uint2*>((E*)p.out + at) = make_uint2(pack<E>(f.x, f.y), pack<E>(f.z, f.w));
+                else *reinterpret_cast<float4*>(to32 + at) = f;
+              }
+            }
+          } else {
+            const int c = col_base + c0 + lane;
+#pragma unroll 8
+            for (int r = 0; r < 32; ++r)
+              if (row_base + r < p.M && c < p.N) {
+                float f = __uint_as_float(lds4(staged(stage, r, lane >> 2) + (lane & 3) * 4));
+                const long long at = (long long)(row_base + r) * p.N + c;
+                if (!p.first) f += acc[at];
+                if (out16) ((E*)p.out)[at] = (E)f;
+                else to32[at] = f;
+              }
+          }
+        }
+      }
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        const unsigned bar = smem_u32(&t.acc_empty[b]);
+        if (CG == 1) ring::mbar_arrive(bar);
+        else arrive_cluster(map_rank(bar, 0));
+      }
+    }
+    if (ROLE == kDz && lane == 0) stores_done();
+  }
+  __syncwarp();
+  tc::fence_before();
+  if (CG == 1) __syncthreads();
+  else cluster_sync();
+  tc::fence_after();
+  if (*abort_flag) {
+    // copies and products that were under way end within microseconds: give them a millisecond before the memory goes
+    if (threadIdx.x == 0) g_head_error = 1;
+    for (int i = 0; i < 50; ++i) __nanosleep(20000);
+    if (CG == 1) __syncthreads();
+  }
+  if (CG == 2) cluster_sync();  // neither block ends while the other may still reach its barriers
+  if (warp == 2) tmem_free<CG>(tmem);
+}
+
+// ------------------------------------------------------------------ operands as the tensor cores take them
+
+template <typename T> __device__ __forceinline__ float as_float(T v) { return (float)v; }
+
+// [rows][width] -> PIECES planes [rows][pitch] of E: fp32 in three bf16 pieces, 16-bit rows on 16 bytes.  target (NULL: all
+// rows count): rows whose target is `ignore` become zeros.
+template <typename T, typename E, int PIECES>
+__global__ void __launch_bounds__(256) lay_out_kernel(const T* __restrict__ src, E* __restrict__ dst, int rows, int width, int pitch,
+                                                      const long long* __restrict__ target, long long ignore) {
+  const long long total = (long long)rows * pitch, plane = total;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const int r = (int)(i / pitch), c = (int)(i - (long long)r * pitch);
+    const bool in = c < width && !(target && target[r] == ignore);
+    const T v = in ? src[(long long)r * width + c] : (T)0.0f;
+    if (PIECES == 1) {
+      dst[i] = (E)v;
+    } else {
+      float left = as_float(v);
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        const E e = (E)left;
+        dst[p * plane + i] = e;
+        left -= as_float(e);
+      }
+    }
+  }
+}
+
+// x with its ignored rows zeroed, where one of them is not finite
+template <typename E>
+__global__ void __launch_bounds__(256) clean_kernel(const E* __restrict__ src, E* __restrict__ dst, int rows, int width,
+                                                    const long long* __restrict__ target, long long ignore,
+                                                    const float* __restrict__ strange) {
+  if (*strange == 0.0f) return;
+  const int pieces = width / 8;
+  const long long total = (long long)rows * pieces;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const bool in = target[i / pieces] != ignore;
+    reinterpret_cast<uint4*>(dst)[i] = in ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ---- sums over splits and rows, in fixed order
+
+struct Join {
+  const float* parts;  // [splits][count]
+  float* acc;
+  void* out;           // NULL: the sum goes to acc
+  long long count;     // 0: nothing to do
+  int splits, first;
+};
+template <typename O>
+__device__ __forceinline__ void join_one(const Join& j, long long i) {
+  float v = j.first ? 0.0f : j.acc[i];
+  for (int s = 0; s < j.splits; ++s) v += j.parts[s * j.count + i];
+  if (j.out) ((O*)j.out)[i] = (O)v;
+  else j.acc[i] = v;
+}
+template <typename O>
+__global__ void __launch_bounds__(256) join_kernel(const Join a, const Join b) {
+  const long long n = a.count + b.count;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    if (i < a.count) join_one<O>(a, i);
+    else join_one<O>(b, i - a.count);
+  }
+}
+
+// db from the sums over 32 rows each: 32 classes a block
+template <typename O>
+__global__ void __launch_bounds__(1024) column_join_kernel(const float* __restrict__ sums, int slabs, int classes, float* acc, O* out,
+                                                           const float* back, int first) {
+  __shared__ float s[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float v = 0;
+  if (c < classes)
+    for (int r = warp; r < slabs; r += 32) v += sums[(long long)r * classes + c];
+  s[warp][lane] = v;
+  __syncthreads();
+  if (warp || c >= classes) return;
+  v = 0;
+  for (int i = 0; i < 32; ++i) v += s[i][lane];
+  if (back) v *= *back;
+  if (!first) v += acc[c];
+  if (out) out[c] = (O)v;
+  else acc[c] = v;
+}
+
+// ------------------------------------------------------------------ plans
+
+struct Config {
+  int cg, bn;
+};
+// Two SMs a tile where their tiles keep half of the pairs busy; below that tiles of one SM, narrow ones when even the wide
+// leave half of the SMs without one.
+Config pick(long long rows, long long cols) {
+  const int sms = device_sm_count();
+  if ((long long)div_up(rows, 256) * div_up(cols, 256) * 4 >= sms) return {2, 256};
+  if ((long long)div_up(rows, 128) * div_up(cols, 128) * 2 >= sms) return {1, 128};
+  return {1, 64};
+}
+int groups_of(const Config& c) { return c.bn >= 128 ? 2 : 1; }
+int clusters_of(const Config& c) { return device_sm_count() / c.cg; }
+
+template <int CG, int BN, int ROLE, typename E, int PIECES>
+int launch_one(const Args& a, int items, cudaStream_t s) {
+  auto kernel = head_kernel<CG, BN, ROLE, E, PIECES>;
+  const int rc = enable_smem(kernel, smem_bytes<CG, BN>());
+  if (rc != DK_OK) return rc;
+  const int clusters = device_sm_count() / CG;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((items < clusters ? items : clusters) * CG), cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem_bytes<CG, BN>(), cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, a);
+  return check_launch();
+}
+template <int ROLE, typename E, int PIECES>
+int launch(const Config& c, const Args& a, int items, cudaStream_t s) {
+  if (c.cg == 2) return launch_one<2, 256, ROLE, E, PIECES>(a, items, s);
+  if (c.bn == 128) return launch_one<1, 128, ROLE, E, PIECES>(a, items, s);
+  return launch_one<1, 64, ROLE, E, PIECES>(a, items, s);
+}
+
+int pieces_of(int dtype) { return dtype == DK_F32 ? 3 : 1; }
+// whether the operands are laid out anew: fp32 always, 16-bit rows that TMA cannot fetch
+bool laid_out(int D, int dtype) { return dtype == DK_F32 || D % 8 != 0; }
+int pitch_of(int n) { return (n + 7) & ~7; }
+
+struct ForwardPlan {
+  Config c;
+  int tiles_m, tiles_n, slots;
+  size_t x, w, top, sum, all, picked, partial, bytes;
+};
+ForwardPlan forward_plan(int T, int D, int V, int dtype) {
+  ForwardPlan p;
+  Layout l;
+  p.c = pick(T, V);
+  p.tiles_m = div_up(T, 128 * p.c.cg), p.tiles_n = div_up(V, p.c.bn), p.slots = p.tiles_n * groups_of(p.c);
+  const bool lay = laid_out(D, dtype);
+  const size_t row = (size_t)pitch_of(D) * 2 * pieces_of(dtype);
+  p.x = lay ? l.take(T * row) : 0, p.w = lay ? l.take(V * row) : 0;
+  const size_t each = (size_t)p.slots * T * sizeof(float);
+  p.top = l.take(each), p.sum = l.take(each), p.all = l.take(each);
+  p.picked = l.take((size_t)T * sizeof(float)), p.partial = l.take(combine_bytes(T));
+  p.bytes = l.bytes;
+  return p;
+}
+
+// dz of one piece; the whole call is one piece where it fits
+constexpr long long kPieceBytes = 128ll << 20;
+
+struct BackwardPlan {
+  Config dz, grad;
+  int tc, vc;                    // rows and classes of a piece: one of them is all there are
+  int splits_w, per_w, splits_x, per_x;
+  size_t x, w, g, back, buffer, acc, acc_b, sums, parts_w, parts_x, bytes;
+};
+
+// splits of the two products so that a launch fills the SMs once where their tiles alone do not
+void split_products(BackwardPlan& p, int D) {
+  const int clusters = clusters_of(p.grad), bm = 128 * p.grad.cg, tn = div_up(D, p.grad.bn);
+  const long long tiles_w = (long long)div_up(p.vc, bm) * tn, tiles_x = (long long)div_up(p.tc, bm) * tn;
+  const int blocks_w = div_up(p.tc, kBox), blocks_x = div_up(p.vc, kBox);
+  const long long total = tiles_w * blocks_w + tiles_x * blocks_x;
+  // at least eight steps a split: less does not pay for writing and joining its sums
+  long long per = total / clusters + 1;
+  if (per < 8) per = 8;
+  p.per_w = (int)(per < blocks_w ? per : blocks_w), p.per_x = (int)(per < blocks_x ? per : blocks_x);
+  p.splits_w = div_up(blocks_w, p.per_w), p.splits_x = div_up(blocks_x, p.per_x);
+  p.per_w = div_up(blocks_w, p.splits_w), p.per_x = div_up(blocks_x, p.splits_x);
+  p.splits_w = div_up(blocks_w, p.per_w), p.splits_x = div_up(blocks_x, p.per_x);
+}
+
+BackwardPlan backward_plan(int T, int D, int V, int dtype) {
+  BackwardPlan p;
+  Layout l;
+  const int pieces = pieces_of(dtype);
+  p.tc = T, p.vc = V;
+  const long long each = 2ll * pieces;
+  if ((long long)T * pitch_of(V) * each > kPieceBytes) {
+    // the longer side is cut: the sums that run over the pieces are those of the shorter one
+    int& side = V >= T ? p.vc : p.tc;
+    const int all = side, other = V >= T ? T : pitch_of(V);
+    long long most = kPieceBytes / (other * each) / 256 * 256;
+    if (most < 256) most = 256;
+    const int n = div_up(all, most);
+    const long long even = (long long)div_up(div_up(all, n), 256) * 256;
+    side = even < all ? (int)even : all;
+  }
+  p.dz = pick(p.tc, p.vc);
+  {
+    // the two products have tc x D and vc x D tiles
+    const int sms = device_sm_count();
+    const long long pairs = (long long)(div_up(p.tc, 256) + div_up(p.vc, 256)) * div_up(D, 256);
+    const long long wide = (long long)(div_up(p.tc, 128) + div_up(p.vc, 128)) * div_up(D, 128);
+    p.grad = pairs * 4 >= sms ? Config{2, 256} : wide * 2 >= sms ? Config{1, 128} : Config{1, 64};
+  }
+  split_products(p, D);
+  const bool lay = laid_out(D, dtype);
+  const size_t row = (size_t)pitch_of(D) * 2 * pieces;
+  p.x = l.take(T * row);  // laid out, or the copy without ignored rows
+  p.w = lay ? l.take(V * row) : 0;
+  p.g = l.take((size_t)T * sizeof(float)), p.back = l.take(2 * sizeof(float));
+  p.buffer = l.take((size_t)p.tc * pitch_of(p.vc) * each);
+  const bool cut_v = p.vc < V, cut_t = p.tc < T;
+  p.acc = (cut_v || cut_t) && dtype != DK_F32 ? l.take((size_t)(cut_v ? T : V) * D * sizeof(float)) : 0;
+  p.acc_b = cut_t ? l.take((size_t)V * sizeof(float)) : 0;
+  p.sums = l.take((size_t)div_up(p.tc, 32) * p.vc * sizeof(float));
+  p.parts_w = p.splits_w > 1 ? l.take((size_t)p.splits_w * p.vc * D * sizeof(float)) : 0;
+  p.parts_x = p.splits_x > 1 ? l.take((size_t)p.splits_x * p.tc * D * sizeof(float)) : 0;
+  p.bytes = l.bytes;
+  return p;
+}
+
+// ------------------------------------------------------------------ calls
+
+unsigned blocks_for(long long n) {
+  const long long b = (n + 255) / 256, most = (long long)device_sm_count() * 8;
+  return (unsigned)(b < most ? b : most);
+}
+
+// tiles of rows whose part of x stays in L2 (126 MB) beside the weights that stream past
+int row_group(const Config& c, int D, int pieces) {
+  const long long g = (40ll << 20) / ((long long)128 * c.cg * D * 2 * pieces);
+  return g < 1 ? 1 : (int)(g > 1 << 20 ? 1 << 20 : g);
+}
+
+// x and w as planes of 16-bit values that TMA can fetch
+template <typename T, typename E, int PIECES>
+int operands(const void*& x, const void*& w, char* to_x, char* to_w, const long long* y, const Shape& h, int dtype, cudaStream_t s) {
+  if (!laid_out(h.D, dtype)) return DK_OK;
+  const int pitch = pitch_of(h.D);
+  lay_out_kernel<T, E, PIECES><<<blocks_for((long long)h.T * pitch), 256, 0, s>>>((const T*)x, (E*)to_x, h.T, h.D, pitch, y, h.ignore);
+  int rc = check_launch();
+  if (rc != DK_OK) return rc;
+  lay_out_kernel<T, E, PIECES><<<blocks_for((long long)h.V * pitch), 256, 0, s>>>((const T*)w, (E*)to_w, h.V, h.D, pitch, nullptr, 0);
+  x = to_x, w = to_w;
+  return check_launch();
+}
+template <typename E, int PIECES>
+bool operand_map(CUtensorMap* tm, const void* p, int rows, int width, int pitch, int box_rows = kBox) {
+  return ring::make_swizzled_map(tm, p, std::is_same<E, __nv_bfloat16>::value, width, rows, PIECES, pitch * 2ll, (long long)rows * pitch * 2,
+                                 box_rows);
+}
+
+template <typename T, typename E, int PIECES>
+int forward(const void* x, const void* w, const void* b, const long long* y, void* loss, void* saved, const Shape& h, int dtype, void* ws,
+            size_t ws_bytes, cudaStream_t s) {
+  const ForwardPlan p = forward_plan(h.T, h.D, h.V, dtype);
+  if (!ws || ws_bytes < p.bytes) return DK_ERR_WORKSPACE;
+  char* m = (char*)ws;
+  int rc = operands<T, E, PIECES>(x, w, m + p.x, m + p.w, y, h, dtype, s);
+  if (rc != DK_OK) return rc;
+  Args a = {};
+  if (!operand_map<E, PIECES>(&a.x, x, h.T, h.D, pitch_of(h.D)) || !operand_map<E, PIECES>(&a.w, w, h.V, h.D, pitch_of(h.D)))
+    return DK_ERR_CUDA;
+  a.rows = h.T, a.classes = h.V, a.depth = div_up(h.D, kBox);
+  a.tiles_m = p.tiles_m, a.tiles_n = p.tiles_n, a.group = row_group(p.c, h.D, PIECES);
+  a.bias = b, a.target = y, a.ignore = h.ignore;
+  a.top = (float*)(m + p.top), a.sum = (float*)(m + p.sum), a.all = h.smoothing != 0.0 ? (float*)(m + p.all) : nullptr;
+  a.picked = (float*)(m + p.picked);
+  if ((long long)p.tiles_m * p.tiles_n > 0x3fffffff) return DK_ERR_UNSUPPORTED;
+  rc = launch<kStats, E, PIECES>(p.c, a, p.tiles_m * p.tiles_n, s);
+  if (rc != DK_OK) return rc;
+  const Partials<float> part = {a.top, a.sum, a.all, a.picked};
+  return launch_combine<float>(part, y, p.slots, loss, saved, (double*)(m + p.partial), h, s);
+}
+
+template <typename T, typename E, int PIECES>
+int backward(const void* up, const void* x, const void* w, const void* b, const long long* y, const void* saved, void* dx, void* dw,
+             void* db, const Shape& h, int dtype, void* ws, size_t ws_bytes, cudaStream_t s) {
+  const BackwardPlan p = backward_plan(h.T, h.D, h.V, dtype);
+  if (!ws || ws_bytes < p.bytes) return DK_ERR_WORKSPACE;
+  char* m = (char*)ws;
+  float *g = (float*)(m + p.g), *back = dtype == DK_F16 ? (float*)(m + p.back) : nullptr;
+  const float* stat = (const float*)saved;
+  int rc = launch_rows<float>(up, y, saved, g, back, h, s);
+  if (rc != DK_OK) return rc;
+  Args a = {};
+  const int pitch = pitch_of(h.D);
+  if (laid_out(h.D, dtype)) {
+    rc = operands<T, E, PIECES>(x, w, m + p.x, m + p.w, y, h, dtype, s);
+  } else if (dw) {
+    a.strange = stat + h.T + 1;
+    clean_kernel<E><<<blocks_for((long long)h.T * h.D / 8), 256, 0, s>>>((const E*)x, (E*)(m + p.x), h.T, h.D, y, h.ignore, a.strange);
+    rc = check_launch();
+  }
+  if (rc != DK_OK) return rc;
+  if (!operand_map<E, PIECES>(&a.x, x, h.T, h.D, pitch) || !operand_map<E, PIECES>(&a.w, w, h.V, h.D, pitch) ||
+      !operand_map<E, PIECES>(&a.x_clean, m + p.x, h.T, h.D, pitch))
+    return DK_ERR_CUDA;
+  a.depth = div_up(h.D, kBox), a.bias = b, a.ignore = h.ignore, a.back = back;
+  a.smooth_each = (float)(h.smoothing / h.V), a.smooth_own = (float)(1.0 - h.smoothing);
+  a.column_sums = db ? (float*)(m + p.sums) : nullptr;
+  const bool cut_v = p.vc < h.V;
+  const int bm = 128 * p.grad.cg, tn = div_up(h.D, p.grad.bn);
+  for (int t0 = 0; t0 < h.T; t0 += p.tc)
+    for (int v0 = 0; v0 < h.V; v0 += p.vc) {
+      const int rows = h.T - t0 < p.tc ? h.T - t0 : p.tc, classes = h.V - v0 < p.vc ? h.V - v0 : p.vc;
+      const bool first_t = t0 == 0, last_t = t0 + rows == h.T, first_v = v0 == 0, last_v = v0 + classes == h.V;
+      const int dz_pitch = pitch_of(classes);
+      if (!operand_map<E, PIECES>(&a.dz, m + p.buffer, rows, classes, dz_pitch) ||
+          !operand_map<E, PIECES>(&a.dz_out, m + p.buffer, rows, classes, dz_pitch, 32))
+        return DK_ERR_CUDA;
+      a.rows = rows, a.classes = classes, a.row0 = t0, a.class0 = v0;
+      a.tiles_m = div_up(rows, 128 * p.dz.cg), a.tiles_n = div_up(classes, p.dz.bn), a.group = row_group(p.dz, h.D, PIECES);
+      a.target = y + t0, a.lse2 = stat + t0, a.g = g + t0;
+      rc = launch<kDz, E, PIECES>(p.dz, a, a.tiles_m * a.tiles_n, s);
+      if (rc != DK_OK) return rc;
+      // dw [classes][D] sums over rows, dx [rows][D] over classes; the running sums of fp32 gradients are the gradients
+      Product pw = {}, px = {};
+      Join jw = {}, jx = {};
+      if (dw) {
+        T* out = (T*)dw + (long long)v0 * h.D;
+        float* acc = PIECES == 3 ? (float*)out : (float*)(m + p.acc);
+        pw.M = classes, pw.N = h.D, pw.blocks = div_up(rows, kBox), pw.tiles_m = div_up(classes, bm), pw.tiles_n = tn;
+        pw.per = p.per_w, pw.splits = div_up(pw.blocks, pw.per);
+        pw.acc = acc, pw.out = last_t ? out : nullptr, pw.first = first_t;
+        if (pw.splits > 1) {
+          jw.parts = (float*)(m + p.parts_w), jw.acc = acc, jw.out = pw.out, jw.count = (long long)classes * h.D;
+          jw.splits = pw.splits, jw.first = first_t;
+          pw.acc = (float*)(m + p.parts_w), pw.out = nullptr, pw.first = 1;
+        }
+      }
+      if (dx) {
+        T* out = (T*)dx + (long long)t0 * h.D;
+        float* acc = PIECES == 3 ? (float*)out : (float*)(m + p.acc);
+        px.M = rows, px.N = h.D, px.blocks = div_up(classes, kBox), px.tiles_m = div_up(rows, bm), px.tiles_n = tn;
+        px.per = p.per_x, px.splits = div_up(px.blocks, px.per);
+        px.acc = acc, px.out = last_v ? out : nullptr, px.first = first_v;
+        if (px.splits > 1) {
+          jx.parts = (float*)(m + p.parts_x), jx.acc = acc, jx.out = px.out, jx.count = (long long)rows * h.D;
+          jx.splits = px.splits, jx.first = first_v;
+          px.acc = (float*)(m + p.parts_x), px.out = nullptr, px.first = 1;
+        }
+      }
+      a.dw = pw, a.dx = px;
+      if (dw || dx) {
+        const long long items = (long long)pw.tiles_m * tn * pw.splits + (long long)px.tiles_m * tn * px.splits;
+        if (items > 0x3fffffff) return DK_ERR_UNSUPPORTED;
+        rc = launch<kGrad, E, PIECES>(p.grad, a, (int)items, s);
+        if (rc != DK_OK) return rc;
+      }
+      if (jw.count + jx.count > 0) {
+        join_kernel<T><<<blocks_for(jw.count + jx.count), 256, 0, s>>>(jw, jx);
+        rc = check_launch();
+        if (rc != DK_OK) return rc;
+      }
+      if (db) {
+        float* acc = cut_v ? nullptr : (float*)(m + p.acc_b);
+        column_join_kernel<T><<<div_up(classes, 32), 1024, 0, s>>>(a.column_sums, div_up(rows, 32), classes, acc,
+                                                                   last_t ? (T*)db + v0 : nullptr, back, first_t);
+        rc = check_launch();
+        if (rc != DK_OK) return rc;
+      }
+    }
+  return DK_OK;
+}
+
+}  // namespace
+
+size_t tc_forward_bytes(int T, int D, int V, int dtype) { return forward_plan(T, D, V, dtype).bytes; }
+size_t tc_backward_bytes(int T, int D, int V, int dtype) { return backward_plan(T, D, V, dtype).bytes; }
+
+int tc_forward(const void* x, const void* w, const void* b, const long long* y, void* loss, void* saved, const Shape& h, int dtype,
+               void* ws, size_t ws_bytes, cudaStream_t s) {
+  switch (dtype) {
+    case DK_F16: return forward<__half, __half, 1>(x, w, b, y, loss, saved, h, dtype, ws, ws_bytes, s);
+    case DK_BF16: return forward<__nv_bfloat16, __nv_bfloat16, 1>(x, w, b, y, loss, saved, h, dtype, ws, ws_bytes, s);
+    default: return forward<float, __nv_bfloat16, 3>(x, w, b, y, loss, saved, h, dtype, ws, ws_bytes, s);
+  }
+}
+
+int tc_backward(const void* up, const void* x, const void* w, const void* b, const long long* y, const void* saved, void* dx, void* dw,
+                void* db, const Shape& h, int dtype, void* ws, size_t ws_bytes, cudaStream_t s) {
+  switch (dtype) {
+    case DK_F16: return backward<__half, __half, 1>(up, x, w, b, y, saved, dx, dw, db, h, dtype, ws, ws_bytes, s);
+    case DK_BF16: return backward<__nv_bfloat16, __nv_bfloat16, 1>(up, x, w, b, y, saved, dx, dw, db, h, dtype, ws, ws_bytes, s);
+    default: return backward<float, __nv_bfloat16, 3>(up, x, w, b, y, saved, dx, dw, db, h, dtype, ws, ws_bytes, s);
+  }
+}
+
+// Code of the last bounded wait that ran out on the current device (0 = none); synchronises with the device.
+int head_error_status() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_head_error, sizeof(int)) != cudaSuccess) return -1;
+  return v;
+}
+
+}  // namespace head
+}  // namespace dk

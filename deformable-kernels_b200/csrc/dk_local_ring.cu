@@ -81,6 +81,18 @@ bool make_plane_row_map(CUtensorMap* tm, const void* base, int elem, int width, 
              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+bool make_swizzled_map(CUtensorMap* tm, const void* base, bool bf16, long long width, long long rows, int planes, long long pitch,
+                       long long plane, int box_rows) {
+  EncodeTiledFn enc = encode_tiled();
+  if (!enc || (reinterpret_cast<uintptr_t>(base) & 15) || (pitch & 15) || (plane & 15)) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)rows, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)pitch, (cuuint64_t)plane};
+  const cuuint32_t box[3] = {64u, (cuuint32_t)box_rows, 1u};
+  const cuuint32_t estr[3] = {1u, 1u, 1u};
+  return enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 }  // namespace ring
 
 namespace {
@@ -1895,7 +1907,8 @@ int local_ring_plan_query(const Geom& g, int pass, long long out[8]) {
 int ring_error_status() {
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_ring_error, sizeof(int)) != cudaSuccess) return -1;
-  return v ? v : tc_error_status();
+  if (!v) v = tc_error_status();
+  return v ? v : head::head_error_status();
 }
 
 // forward (transposed = false) or grad-input (transposed = true); DK_ERR_UNSUPPORTED = not a ring shape

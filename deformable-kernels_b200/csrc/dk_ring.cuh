@@ -86,6 +86,11 @@ __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* tm) {
 bool make_plane_row_map(CUtensorMap* tm, const void* base, int elem, int width, int rows, long long planes, int box_w,
                         int box_planes);
 
+// 16-bit values [planes][rows][width] with `pitch` bytes from row to row (a multiple of 16) and `plane` bytes from plane to
+// plane; one box = 64 values of `box_rows` rows, 128 swizzled bytes a row in shared memory.  false: TMA cannot fetch it.
+bool make_swizzled_map(CUtensorMap* tm, const void* base, bool bf16, long long width, long long rows, int planes, long long pitch,
+                       long long plane, int box_rows);
+
 // Bookkeeping of one ring of n slots (any n from 2 up, not only powers of two: shared memory decides the depth).
 // Fill number k goes to slot k mod n and is phase k / n ("turn") of that slot's two barriers.  A phase can only
 // be told from its parity, so a consumer may wait on the "full" barrier of fill k only once the slot has been

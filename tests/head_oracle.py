@@ -59,12 +59,19 @@ def dropout(x, p, seed, offset=0, shared_dims=0):
 
 # ------------------------------------------------------------------ linear layer + cross entropy
 
-def head(x, w, y, b=None, up=None, ignore_index=-100, reduction="mean", label_smoothing=0.0):
-    """Loss and gradients in 64 bits, and the bounds of their errors: ({name: value}, {name: bound})."""
+def head(x, w, y, b=None, up=None, ignore_index=-100, reduction="mean", label_smoothing=0.0, device="cpu"):
+    """Loss and gradients in 64 bits, and the bounds of their errors: ({name: value}, {name: bound}), on the CPU; `device`:
+    where they are computed."""
+    with torch.device(device):
+        out, far = _head(x.to(device), w.to(device), y.to(device), b.to(device) if b is not None else None,
+                         up.to(device) if up is not None else None, ignore_index, reduction, label_smoothing)
+    return {k: v.cpu() for k, v in out.items()}, {k: v.cpu() for k, v in far.items()}
+
+
+def _head(x, w, y, b, up, ignore_index, reduction, label_smoothing):
     dtype = x.dtype
-    x, w = x.double().cpu(), w.double().cpu()
-    b = b.double().cpu() if b is not None else None
-    y = y.cpu()
+    x, w = x.double(), w.double()
+    b = b.double() if b is not None else None
     t, d = x.shape
     v = w.shape[0]
     s = label_smoothing
@@ -92,7 +99,7 @@ def head(x, w, y, b=None, up=None, ignore_index=-100, reduction="mean", label_sm
            (row_err + 4 * step * each.abs()).sum() / (count if reduction == "mean" else 1)}
     if up is None:
         return out, far
-    up = up.double().cpu()
+    up = up.double()
     g = torch.where(live, up / count if reduction == "mean" else up * torch.ones(t, dtype=torch.double), torch.zeros((), dtype=torch.double))
     p = torch.exp(z - lse[:, None])
     dz = p - s / v

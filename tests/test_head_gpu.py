@@ -13,6 +13,13 @@ def functions():
     return f
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    from deformable_kernels import _cabi
+    assert _cabi.lib.dk_ring_error_status() == 0
+
+
 # ------------------------------------------------------------------ dropout
 
 @pytest.mark.parametrize("dtype", list(H.DTYPES))
@@ -121,12 +128,12 @@ def make(t, d, v, dtype, bias=True, ignored=0.0, reduction="mean", seed=0):
     return x, w, y, b, up.double() if dtype == "fp64" else up
 
 
-def check(x, w, y, b, up, where="", **kw):
+def check(x, w, y, b, up, where="", device="cpu", **kw):
     """One call and its gradients against the 64-bit oracle, every value within its bound."""
     leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b) if t is not None]
     loss = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), leaves[2] if b is not None else None, **kw)
     grads = torch.autograd.grad(loss, leaves, up.to(DEV))
-    out, far = H.head(x, w, y, b, up, **kw)
+    out, far = H.head(x, w, y, b, up, device=device, **kw)
     got = dict(zip(("loss", "dx", "dw", "db"), (loss.detach(),) + grads))
     assert loss.dtype == (torch.float64 if x.dtype == torch.float64 else torch.float32)
     for name, v in got.items():
@@ -149,6 +156,16 @@ SIZES = [(1, 8, 2), (1, 1280, 1000), (2, 1, 1), (31, 24, 7), (33, 33, 65), (127,
 @pytest.mark.parametrize("t, d, v", SIZES)
 def test_head_sizes(t, d, v, dtype):
     check(*make(t, d, v, dtype, seed=t + d + v))
+
+
+# tiles shared by two SMs, in one or all products; several pieces of the classes, of the rows; long sums that are split
+LARGE = [(2100, 72, 5000), (1500, 520, 4600), (3000, 136, 24100), (24100, 40, 3001), (9000, 64, 40), (20, 72, 30000), (4700, 1032, 600)]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("t, d, v", LARGE)
+def test_head_large_sizes(t, d, v, dtype):
+    check(*make(t, d, v, dtype, ignored=0.1, seed=t + d + v), device=DEV, label_smoothing=0.1)
 
 
 @pytest.mark.parametrize("dtype", list(H.DTYPES))
