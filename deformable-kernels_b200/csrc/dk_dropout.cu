@@ -26,14 +26,34 @@ struct DropArgs {
   unsigned long long* used;        // device or NULL: where the seed and offset of this call are kept for its backward
   unsigned hi, lo;                 // threshold: upper 16 bits (65536: nothing is kept), lower 16 bits
   double scale;
+  unsigned long long first_group;  // of this launch: groups of eight elements, all with the same upper 32 bits
+  unsigned groups;
 };
 
 struct Key {
   unsigned k0, k1, o0, o1;
 };
 
-__device__ __forceinline__ uint4 philox(unsigned long long group, unsigned second, const Key& k) {
-  unsigned c0 = (unsigned)group, c1 = (unsigned)(group >> 32) | second, c2 = k.o0, c3 = k.o1;
+// The generator's key, kept for the backward where that is wanted.  As 32-bit words that are loaded without a condition it stays in
+// uniform registers, its ten round keys with it: 104 us against 127 (154 M fp16 values).
+template <bool STATE>
+__device__ __forceinline__ Key key_of(const DropArgs& a) {
+  const unsigned add0 = (unsigned)a.offset, add1 = (unsigned)(a.offset >> 32);
+  Key k = {(unsigned)a.seed, (unsigned)(a.seed >> 32), add0, add1};
+  if (STATE) {
+    const unsigned* s = reinterpret_cast<const unsigned*>(a.state);
+    const unsigned o0 = s[2], o1 = s[3], sum = o0 + add0;
+    k = {s[0], s[1], sum, o1 + add1 + (sum < o0 ? 1u : 0u)};
+    if (a.used && blockIdx.x == 0 && threadIdx.x == 0) {
+      unsigned* u = reinterpret_cast<unsigned*>(a.used);
+      u[0] = k.k0, u[1] = k.k1, u[2] = k.o0, u[3] = k.o1;
+    }
+  }
+  return k;
+}
+
+__device__ __forceinline__ uint4 philox(unsigned c0, unsigned c1, const Key& k) {
+  unsigned c2 = k.o0, c3 = k.o1;
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
@@ -47,104 +67,180 @@ __device__ __forceinline__ unsigned half_word(const uint4& w, int i) {
   const unsigned v = (i & 4) ? ((i & 2) ? w.w : w.z) : ((i & 2) ? w.y : w.x);
   return (i & 1) ? v >> 16 : v & 0xffffu;
 }
-// u: the upper half of draw 8 group + i
-__device__ __forceinline__ bool kept(unsigned u, unsigned long long group, int i, const Key& k, unsigned hi, unsigned lo) {
-  if (u != hi) return u > hi;
-  return lo == 0 || half_word(philox(group, 0x80000000u, k), i) >= lo;
+// bit i: draw 8 group + i is kept; any threshold
+__device__ __forceinline__ unsigned kept8(unsigned long long group, const Key& k, unsigned hi, unsigned lo) {
+  const unsigned c0 = (unsigned)group, c1 = (unsigned)(group >> 32);
+  const uint4 w = philox(c0, c1, k);
+  unsigned keep = 0, even = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const unsigned u = half_word(w, i);
+    keep |= (unsigned)(u > hi) << i;
+    even |= (unsigned)(u == hi) << i;
+  }
+  if (even) {
+    const uint4 l = philox(c0, c1 | 0x80000000u, k);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) keep |= (even >> i & 1 & (unsigned)(half_word(l, i) >= lo)) << i;
+  }
+  return keep;
 }
 
-template <typename T> struct Value {
-  using A = typename Compute<T>::type;
-  static __device__ __forceinline__ T times(T v, A s) { return (T)((A)v * s); }
-};
-template <> struct Value<__half> {
-  using A = float;
-  static __device__ __forceinline__ __half times(__half v, float s) { return __float2half_rn(__half2float(v) * s); }
-};
-template <> struct Value<__nv_bfloat16> {
-  using A = float;
-  static __device__ __forceinline__ __nv_bfloat16 times(__nv_bfloat16 v, float s) { return __float2bfloat16_rn(__bfloat162float(v) * s); }
-};
+__device__ __forceinline__ unsigned settled(unsigned w, unsigned low, unsigned both, unsigned lo) {
+  const unsigned d = w ^ both;
+  if ((d & 0xffffu) == 0) w = (w & 0xffff0000u) | ((low & 0xffffu) >= lo ? 0xffffu : 0u);
+  if ((d >> 16) == 0) w = (w & 0xffffu) | ((low >> 16) >= lo ? 0xffff0000u : 0u);
+  return w;
+}
+// The upper halves of draws 8 group ... + 7, moved off the threshold: one that equals it becomes the lowest or the highest, as
+// the draw's lower half says.  `both`: the threshold's upper half twice, below 0xffff.
+__device__ __forceinline__ uint4 draws8(unsigned c0, unsigned c1, const Key& k, unsigned both, unsigned lo) {
+  uint4 w = philox(c0, c1, k);
+  // a half word that is zero sets its highest bit (so may the one above it: `settled` looks again)
+  const unsigned a = w.x ^ both, b = w.y ^ both, c = w.z ^ both, d = w.w ^ both;
+  const unsigned even = ((a - 0x00010001u) & ~a) | ((b - 0x00010001u) & ~b) | ((c - 0x00010001u) & ~c) | ((d - 0x00010001u) & ~d);
+  if (even & 0x80008000u) {
+    const uint4 l = philox(c0, c1 | 0x80000000u, k);
+    w.x = settled(w.x, l.x, both, lo), w.y = settled(w.y, l.y, both, lo), w.z = settled(w.z, l.z, both, lo);
+    w.w = settled(w.w, l.w, both, lo);
+  }
+  return w;
+}
 
-// A thread takes eight consecutive elements at a time: one counter's worth of draws when every element has its own.
-// VECTOR: both tensors begin on 16 bytes.  SHARED: run > 1; at most two counters for eight elements, and elements whose
-// run is dropped are not read.
-template <typename T, bool VECTOR, bool SHARED>
-__global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, T* __restrict__ y, const DropArgs a) {
+// Sixteen bytes of values: what is kept times the scale, zeros elsewhere.  16-bit values are converted and rounded in pairs, which the
+// conversion units do at twice the rate.
+template <typename T> struct Piece {
+  static __device__ __forceinline__ void apply(uint4& v, float s, const bool* k);
+};
+template <> struct Piece<float> {
+  static __device__ __forceinline__ void apply(uint4& v, float s, const bool* k) {
+    v.x = k[0] ? __float_as_uint(__uint_as_float(v.x) * s) : 0u, v.y = k[1] ? __float_as_uint(__uint_as_float(v.y) * s) : 0u;
+    v.z = k[2] ? __float_as_uint(__uint_as_float(v.z) * s) : 0u, v.w = k[3] ? __float_as_uint(__uint_as_float(v.w) * s) : 0u;
+  }
+};
+template <> struct Piece<double> {
+  static __device__ __forceinline__ void apply(uint4& v, double s, const bool* k) {
+    double a = __hiloint2double((int)v.y, (int)v.x), b = __hiloint2double((int)v.w, (int)v.z);
+    a = k[0] ? a * s : 0.0, b = k[1] ? b * s : 0.0;
+    v = make_uint4((unsigned)__double2loint(a), (unsigned)__double2hiint(a), (unsigned)__double2loint(b), (unsigned)__double2hiint(b));
+  }
+};
+__device__ __forceinline__ unsigned pair_of(unsigned v, float s, bool k0, bool k1, __half) {
+  float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  f.x = k0 ? f.x * s : 0.0f, f.y = k1 ? f.y * s : 0.0f;
+  const __half2 h = __float22half2_rn(f);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ unsigned pair_of(unsigned v, float s, bool k0, bool k1, __nv_bfloat16) {
+  float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+  f.x = k0 ? f.x * s : 0.0f, f.y = k1 ? f.y * s : 0.0f;
+  const __nv_bfloat162 h = __float22bfloat162_rn(f);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ void Piece<T>::apply(uint4& v, float s, const bool* k) {
+  v.x = pair_of(v.x, s, k[0], k[1], T()), v.y = pair_of(v.y, s, k[2], k[3], T());
+  v.z = pair_of(v.z, s, k[4], k[5], T()), v.w = pair_of(v.w, s, k[6], k[7], T());
+}
+template <typename T, typename A> __device__ __forceinline__ T times(T v, A s) { return (T)((A)v * s); }
+template <> __device__ __forceinline__ __half times<__half, float>(__half v, float s) { return __float2half_rn(__half2float(v) * s); }
+template <> __device__ __forceinline__ __nv_bfloat16 times<__nv_bfloat16, float>(__nv_bfloat16 v, float s) {
+  return __float2bfloat16_rn(__bfloat162float(v) * s);
+}
+
+// Every element has its own draw; both tensors begin on 16 bytes, hold whole groups of eight (the elements of this launch), and the
+// threshold's upper half is below 0xffff.  A thread takes eight elements at a time, one counter's worth of draws.  All the warps an SM can hold, with registers to match, hide the
+// generator's latency: 102 us against 123 with the registers that ptxas takes by itself.
+template <typename T, bool STATE>
+__global__ void __launch_bounds__(256, 8) dropout_kernel(const T* __restrict__ x, T* __restrict__ y, const DropArgs a) {
   constexpr int kPieces = 8 * sizeof(T) / 16;
-  using A = typename Value<T>::A;
-  unsigned long long seed = a.seed, offset = a.offset;
-  if (a.state) seed = a.state[0], offset += a.state[1];
-  if (a.used && blockIdx.x == 0 && threadIdx.x == 0) a.used[0] = seed, a.used[1] = offset;
-  const Key key = {(unsigned)seed, (unsigned)(seed >> 32), (unsigned)offset, (unsigned)(offset >> 32)};
+  using A = typename Compute<T>::type;
+  const Key key = key_of<STATE>(a);
   const A scale = (A)a.scale;
-  const T zero = (T)0.0f;
-  const unsigned long long groups = (a.count + 7) >> 3, step = (unsigned long long)gridDim.x * blockDim.x;
-  for (unsigned long long g = (unsigned long long)blockIdx.x * blockDim.x + threadIdx.x; g < groups; g += step) {
-    const unsigned long long first = g << 3;
+  // as upper half of a word a draw is above these whatever the lower half holds, as lower half after a shift
+  const unsigned above_hi = a.hi << 16 | 0xffffu, above_lo = a.hi << 16, both = a.hi * 0x00010001u;
+  for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < a.groups; i += gridDim.x * 256) {
+    uint4 v[kPieces];
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q) v[q] = __ldg(reinterpret_cast<const uint4*>(x) + (size_t)i * kPieces + q);
+    const uint4 w = draws8((unsigned)a.first_group + i, (unsigned)(a.first_group >> 32), key, both, a.lo);
+    const bool k[8] = {w.x << 16 > above_lo, w.x > above_hi, w.y << 16 > above_lo, w.y > above_hi,
+                       w.z << 16 > above_lo, w.z > above_hi, w.w << 16 > above_lo, w.w > above_hi};
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q) {
+      Piece<T>::apply(v[q], scale, k + q * (8 / kPieces));
+      reinterpret_cast<uint4*>(y)[(size_t)i * kPieces + q] = v[q];
+    }
+  }
+}
+
+// The same for tensors that begin elsewhere (VECTOR = false), for runs of elements that share a draw (those that are dropped are
+// not read), and for any threshold.
+template <typename T, bool VECTOR, bool STATE>
+__global__ void __launch_bounds__(256) dropout_runs_kernel(const T* __restrict__ x, T* __restrict__ y, const DropArgs a) {
+  constexpr int kPieces = 8 * sizeof(T) / 16;
+  using A = typename Compute<T>::type;
+  const Key key = key_of<STATE>(a);
+  const A scale = (A)a.scale;
+  for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < a.groups; i += gridDim.x * 256) {
+    const unsigned long long g = a.first_group + i, first = g << 3;
     const int n = a.count - first < 8 ? (int)(a.count - first) : 8;
-    unsigned keep = 0;
-    if (!SHARED) {
-      const uint4 w = philox(g, 0, key);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) keep |= (unsigned)kept(half_word(w, i), g, i, key, a.hi, a.lo) << i;
+    unsigned long long j = a.run == 1 ? first : first / a.run;
+    unsigned long long left = a.run - (first - j * a.run);  // elements of run j from here on
+    unsigned keep = 0, eight = kept8(j >> 3, key, a.hi, a.lo);
+    if (a.run == 1) {
+      keep = eight;
+    } else if (left >= 8) {
+      keep = (eight >> (j & 7) & 1) ? 0xffu : 0u;
     } else {
-      unsigned long long j = first / a.run;
-      unsigned long long left = a.run - (first - j * a.run);  // elements of run j from here on
-      unsigned long long have = ~0ull;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      bool k = false;
-      bool fresh = true;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (left == 0) ++j, left = a.run, fresh = true;
-        if (fresh && i < n) {
-          if (j >> 3 != have) have = j >> 3, w = philox(have, 0, key);
-          k = kept(half_word(w, (int)(j & 7)), have, (int)(j & 7), key, a.hi, a.lo);
-          fresh = false;
+      for (int e = 0; e < n; ++e, --left) {
+        if (left == 0) {
+          ++j, left = a.run;
+          if ((j & 7) == 0) eight = kept8(j >> 3, key, a.hi, a.lo);
         }
-        --left;
-        keep |= (unsigned)k << i;
+        keep |= (eight >> (j & 7) & 1) << e;
       }
     }
     if (VECTOR && n == 8) {
-      alignas(16) T v[8];
-      if (!SHARED || keep) {
+      bool k[8];
 #pragma unroll
-        for (int q = 0; q < kPieces; ++q) reinterpret_cast<uint4*>(v)[q] = __ldg(reinterpret_cast<const uint4*>(x + first) + q);
-      } else {
+      for (int e = 0; e < 8; ++e) k[e] = keep >> e & 1;
 #pragma unroll
-        for (int q = 0; q < kPieces; ++q) reinterpret_cast<uint4*>(v)[q] = make_uint4(0, 0, 0, 0);
+      for (int q = 0; q < kPieces; ++q) {
+        uint4 v = keep ? __ldg(reinterpret_cast<const uint4*>(x + first) + q) : make_uint4(0, 0, 0, 0);
+        Piece<T>::apply(v, scale, k + q * (8 / kPieces));
+        reinterpret_cast<uint4*>(y + first)[q] = v;
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = (keep >> i & 1) ? Value<T>::times(v[i], scale) : zero;
-#pragma unroll
-      for (int q = 0; q < kPieces; ++q) reinterpret_cast<uint4*>(y + first)[q] = reinterpret_cast<const uint4*>(v)[q];
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) y[first + i] = (keep >> i & 1) ? Value<T>::times(x[first + i], scale) : zero;
+      for (int e = 0; e < 8; ++e)
+        if (e < n) y[first + e] = (keep >> e & 1) ? times<T, A>(x[first + e], scale) : (T)0.0f;
     }
   }
 }
 
-template <typename T>
-int launch_dropout(const void* input, void* output, const DropArgs& a, cudaStream_t s) {
+template <typename T, bool STATE>
+int launch_dropout(const void* input, void* output, DropArgs a, cudaStream_t s) {
   const T* x = (const T*)input;
   T* y = (T*)output;
   const bool vector = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0;
-  const unsigned long long blocks = (((a.count + 7) >> 3) + 255) >> 8;
-  // 16 blocks per SM and a loop: 102 us where a block per 2048 elements takes 111 (154 M fp16 values)
-  const unsigned long long most = (unsigned long long)device_sm_count() * 16;
-  const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-  if (a.run == 1) {
-    if (vector) dropout_kernel<T, true, false><<<grid, 256, 0, s>>>(x, y, a);
-    else dropout_kernel<T, false, false><<<grid, 256, 0, s>>>(x, y, a);
-  } else {
-    if (vector) dropout_kernel<T, true, true><<<grid, 256, 0, s>>>(x, y, a);
-    else dropout_kernel<T, false, true><<<grid, 256, 0, s>>>(x, y, a);
+  const unsigned most = (unsigned)device_sm_count() * 32;
+  unsigned long long at = 0, total = (a.count + 7) >> 3;
+  while (at < total) {
+    unsigned long long n = total - at < 1ull << 30 ? total - at : 1ull << 30;
+    // whole groups first, an incomplete one by itself: looking for it in the kernel costs every group a tenth of its time
+    const bool whole = a.run == 1 && vector && a.hi < 0xffffu && (a.count >> 3) > at;
+    if (whole && n > (a.count >> 3) - at) n = (a.count >> 3) - at;
+    a.first_group = at, a.groups = (unsigned)n;
+    const unsigned blocks = (a.groups + 255) >> 8, grid = blocks < most ? blocks : most;
+    if (whole) dropout_kernel<T, STATE><<<grid, 256, 0, s>>>(x + (at << 3), y + (at << 3), a);
+    else if (vector) dropout_runs_kernel<T, true, STATE><<<grid, 256, 0, s>>>(x, y, a);
+    else dropout_runs_kernel<T, false, STATE><<<grid, 256, 0, s>>>(x, y, a);
+    const int rc = check_launch();
+    if (rc != DK_OK) return rc;
+    at += n;
   }
-  return check_launch();
+  return DK_OK;
 }
 
 }  // namespace
@@ -154,9 +250,9 @@ using namespace dk;
 
 extern "C" int dk_dropout(const void* input, void* output, long long count, long long run, double p, unsigned long long seed,
                           unsigned long long offset, const void* state, void* used, int dtype, void* stream) {
-  if (!input || !output || count <= 0 || run <= 0 || !(p >= 0.0 && p <= 1.0)) return DK_ERR_BAD_ARGUMENT;
+  if (!input || !output || count <= 0 || run <= 0 || !(p >= 0.0 && p <= 1.0) || (used && !state)) return DK_ERR_BAD_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(state) | reinterpret_cast<uintptr_t>(used)) & 7) return DK_ERR_BAD_ARGUMENT;
-  DropArgs a;
+  DropArgs a = {};
   a.count = (unsigned long long)count, a.run = (unsigned long long)run;
   a.seed = seed, a.offset = offset;
   a.state = (const unsigned long long*)state, a.used = (unsigned long long*)used;
@@ -165,10 +261,10 @@ extern "C" int dk_dropout(const void* input, void* output, long long count, long
   a.scale = p < 1.0 ? 1.0 / (1.0 - p) : 0.0;
   cudaStream_t s = (cudaStream_t)stream;
   switch (dtype) {
-    case DK_F32: return launch_dropout<float>(input, output, a, s);
-    case DK_F16: return launch_dropout<__half>(input, output, a, s);
-    case DK_BF16: return launch_dropout<__nv_bfloat16>(input, output, a, s);
-    case DK_F64: return launch_dropout<double>(input, output, a, s);
+    case DK_F32: return state ? launch_dropout<float, true>(input, output, a, s) : launch_dropout<float, false>(input, output, a, s);
+    case DK_F16: return state ? launch_dropout<__half, true>(input, output, a, s) : launch_dropout<__half, false>(input, output, a, s);
+    case DK_BF16: return state ? launch_dropout<__nv_bfloat16, true>(input, output, a, s) : launch_dropout<__nv_bfloat16, false>(input, output, a, s);
+    case DK_F64: return state ? launch_dropout<double, true>(input, output, a, s) : launch_dropout<double, false>(input, output, a, s);
     default: return DK_ERR_BAD_ARGUMENT;
   }
 }

@@ -75,7 +75,7 @@ def test_library_refuses_bad_calls_before_any_launch():
         return C.lib.dk_dropout(x, y, count, run, p, 0, 0, state, used, dtype, null)
     assert drop(x=null) == 1 and drop(y=null) == 1 and drop(count=0) == 1 and drop(run=0) == 1 and drop(dtype=4) == 1
     assert drop(p=-0.1) == 1 and drop(p=1.1) == 1 and drop(p=float("nan")) == 1
-    assert drop(state=ctypes.c_void_p(12)) == 1 and drop(used=ctypes.c_void_p(20)) == 1
+    assert drop(state=ctypes.c_void_p(12)) == 1 and drop(state=one, used=ctypes.c_void_p(20)) == 1 and drop(used=one) == 1
 
     def forward(x=one, w=one, y=one, loss=one, rows=2, features=8, classes=3, reduction=1, smoothing=0.0, dtype=0, ws=null, size=0):
         return C.lib.dk_linear_cross_entropy_forward(x, w, null, y, loss, null, rows, features, classes, -100, reduction, smoothing, dtype,
