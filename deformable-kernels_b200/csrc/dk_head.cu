@@ -6,17 +6,21 @@
 //   dz_tv = g_t (exp(z_tv - lse_t) - (1 - s) [v = y_t] - s / V)     g_t: what arrives from behind the loss
 //   dx = dz W,   dW = dz^T x,   db = sum_t dz_t
 //
-// Forward: tiles of logits live in registers only; each leaves (maximum, sum of exponentials) of its rows, kept to the
-// base 2, and a second kernel joins the tiles of a row in fixed order.  Backward: a piece of the vocabulary at a time, the
+// Forward: tiles of logits live in registers only; each leaves (maximum, sum of exponentials) of its rows, and a second
+// kernel joins the tiles of a row in fixed order.  Backward: a piece of the vocabulary at a time, the
 // logits of the piece once more, dz of the piece into the workspace, then the two products.
 //
-// Here: the C entry points, the small kernels, and kernels on the CUDA cores for every type.
+// Here: the C entry points, the kernel that joins a row's tiles, and fp64 on the CUDA cores.  The other types: dk_head_tc.cu.
 #include <math_constants.h>
 
 #include "dk_head.cuh"
 
 namespace dk {
 namespace head {
+
+// e^v of differences that are not above zero
+__device__ __forceinline__ double power(double v) { return exp(v); }
+__device__ __forceinline__ float power(float v) { return exp2f(v * (float)kLog2e); }
 
 template <typename A> __device__ __forceinline__ A minus_inf() { return (A)-CUDART_INF_F; }
 
@@ -64,7 +68,8 @@ __device__ __forceinline__ double sum16(double v) {
 
 __global__ void __launch_bounds__(256) logits_stats_kernel(const double* __restrict__ x, const double* __restrict__ w,
                                                            const double* __restrict__ b, const long long* __restrict__ y,
-                                                           Partials<double> p, Shape h) {
+                                                           Partials<double> p, unsigned* count, Shape h) {
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *count = 0;
   __shared__ double sx[kDepth * kPitch], sw[kDepth * kPitch];
   const int r0 = blockIdx.y * kTile, c0 = blockIdx.x * kTile;
   double z[4][4];
@@ -82,7 +87,6 @@ __global__ void __launch_bounds__(256) logits_stats_kernel(const double* __restr
         if (b) z[i][j] += b[c];
         if (yr == c) p.picked[r] = z[i][j];
         all += z[i][j];
-        z[i][j] *= kLog2e;
       } else {
         z[i][j] = minus_inf<double>();
       }
@@ -92,7 +96,7 @@ __global__ void __launch_bounds__(256) logits_stats_kernel(const double* __restr
     const double ref = top == minus_inf<double>() ? 0 : top;
     double sum = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum += exp2(z[i][j] - ref);
+    for (int j = 0; j < 4; ++j) sum += exp(z[i][j] - ref);
     sum = sum16(sum);
     all = sum16(all);
     if (tx == 0 && r < h.T) {
@@ -106,8 +110,7 @@ __global__ void __launch_bounds__(256) logits_stats_kernel(const double* __restr
 // dz of the classes [v0, v0 + vc)
 __global__ void __launch_bounds__(256) logits_dz_kernel(const double* __restrict__ x, const double* __restrict__ w,
                                                         const double* __restrict__ b, const long long* __restrict__ y,
-                                                        const double* __restrict__ lse2, const double* __restrict__ g,
-                                                        double* __restrict__ dz, int v0, int vc, Shape h) {
+                                                        const double* __restrict__ saved, Upstream<double> up, double* __restrict__ dz, int v0, int vc, Shape h) {
   __shared__ double sx[kDepth * kPitch], sw[kDepth * kPitch];
   const int r0 = blockIdx.y * kTile, c0 = v0 + blockIdx.x * kTile;
   double z[4][4];
@@ -118,13 +121,13 @@ __global__ void __launch_bounds__(256) logits_dz_kernel(const double* __restrict
     const int r = r0 + 4 * ty + i;
     if (r >= h.T) continue;
     const long long yr = y[r];
-    const double l2 = lse2[r], gr = g[r];
+    const double ref = saved[r], inv = saved[h.T + r], gr = upstream_row(up, r, yr, h.ignore, h.V) * upstream_back(up);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = c0 + 4 * tx + j;
       if (c >= v0 + vc) continue;
       if (b) z[i][j] += b[c];
-      double d = exp2(z[i][j] * kLog2e - l2) - h.smoothing / h.V;
+      double d = exp(z[i][j] - ref) * inv - h.smoothing / h.V;
       if (yr == c) d -= 1.0 - h.smoothing;
       // an ignored row has no gradient, whatever its logits are
       dz[(long long)r * vc + c - v0] = yr == h.ignore ? 0 : d * gr;
@@ -182,22 +185,155 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const double* __restri
   out[c] = v;
 }
 
+// ------------------------------------------------------------------ a few rows
+
+// eight values, beginning on 16 bytes
+template <typename T> __device__ __forceinline__ void load8(float (&v)[8], const T* p);
+template <> __device__ __forceinline__ void load8<float>(float (&v)[8], const float* p) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+template <> __device__ __forceinline__ void load8<__half>(float (&v)[8], const __half* p) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+  const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+template <> __device__ __forceinline__ void load8<__nv_bfloat16>(float (&v)[8], const __nv_bfloat16* p) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+  const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+
+// R rows of x (h.T of them exist), read again and again from L1; a warp takes C classes at a time, its lanes share the features, lane r keeps
+// the statistics of row r.  One slot a block.
+template <typename T, int R, int C>
+__global__ void __launch_bounds__(256, R * C <= 8 ? 4 : 2) few_rows_kernel(const T* __restrict__ x, const T* __restrict__ w,
+                                                                          const T* __restrict__ b, const long long* __restrict__ y,
+                                                                          Partials<float> p, unsigned* count, Shape h) {
+  __shared__ float s_top[8][R], s_sum[8][R], s_all[8][R];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  before_all();
+  let_next();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *count = 0;
+  const long long own = lane < h.T && lane < R ? y[lane] : -1;
+  const T* from[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) from[r] = x + (long long)(r < h.T ? r : 0) * h.D;
+  float top = minus_inf<float>(), sum = 0, all = 0;
+  for (int c0 = (blockIdx.x * 8 + warp) * C; c0 < h.V; c0 += gridDim.x * 8 * C) {
+    float acc[C][R] = {};
+    const T* row[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) row[c] = w + (long long)(c0 + c < h.V ? c0 + c : c0) * h.D;
+    if (h.D % 8 == 0) {
+#pragma unroll(R * C <= 4 ? 4 : 1)
+      for (int k = lane * 8; k < h.D; k += 256) {
+        float wv[C][8];
+#pragma unroll
+        for (int c = 0; c < C; ++c) load8<T>(wv[c], row[c] + k);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float xv[8];
+          load8<T>(xv, from[r] + k);
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[c][r] += wv[c][e] * xv[e];
+        }
+      }
+    } else {
+      for (int k = lane; k < h.D; k += 32)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const float v = (float)row[c][k];
+#pragma unroll
+          for (int r = 0; r < R; ++r) acc[c][r] += v * (float)from[r][k];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float z = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float v = acc[c][r];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == r) z = v;
+      }
+      if (c0 + c < h.V) {
+        if (b) z += (float)b[c0 + c];
+        if (own == c0 + c) p.picked[lane] = z;
+        all += z;
+        const float n = fmaxf(top, z), ref = n == minus_inf<float>() ? 0.0f : n;
+        sum = sum * power(top - ref) + power(z - ref);
+        top = n;
+      }
+    }
+  }
+  if (lane < R) s_top[warp][lane] = top, s_sum[warp][lane] = sum, s_all[warp][lane] = all;
+  __syncthreads();
+  if (threadIdx.x >= R || threadIdx.x >= h.T) return;
+  top = minus_inf<float>(), sum = 0, all = 0;
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, s_top[i][lane]);
+  const float ref = top == minus_inf<float>() ? 0.0f : top;
+  for (int i = 0; i < 8; ++i) sum += s_sum[i][lane] * power(s_top[i][lane] - ref), all += s_all[i][lane];
+  const long long at = (long long)blockIdx.x * h.T + lane;
+  p.top[at] = top, p.sum[at] = sum;
+  if (h.smoothing != 0.0) p.all[at] = all;
+}
+
+// 16-bit weights: four rows take 10.2 / 25.6 / 77.8 us here and 12.5 / 28.7 / 77.8 on the tensor cores (1000 and 21841 classes of 1280 features, 65536 of
+// 2048), eight 10.4 / 34.8 / 114.  fp32 weights, which the tensor cores want laid out in pieces first: eight rows 12.3 / 53.6 / 162 and 30.7 / 127 / 567.
+bool few_rows(int T, int dtype) { return T <= (dtype == DK_F32 ? 8 : 4); }
+// one class a warp, four where there are enough of them
+static bool four_classes(int V) { return V >= device_sm_count() * 8 * 4; }
+int few_slots(int V) {
+  const int blocks = div_up(V, 8 * (four_classes(V) ? 4 : 1)), most = device_sm_count() * 4;
+  return blocks < most ? blocks : most;
+}
+template <typename T, int R>
+static int launch_few(const void* x, const void* w, const void* b, const long long* y, const Partials<float>& p, unsigned* count,
+                      const Shape& h, cudaStream_t s) {
+  return launch_after(four_classes(h.V) ? few_rows_kernel<T, R, 4> : few_rows_kernel<T, R, 1>, few_slots(h.V), 256, 0, 1, s, (const T*)x,
+                      (const T*)w, (const T*)b, y, p, count, h);
+}
+template <typename T>
+int launch_few_rows(const void* x, const void* w, const void* b, const long long* y, const Partials<float>& p, unsigned* count,
+                    const Shape& h, cudaStream_t s) {
+  if (h.T == 1) return launch_few<T, 1>(x, w, b, y, p, count, h, s);
+  if (h.T == 2) return launch_few<T, 2>(x, w, b, y, p, count, h, s);
+  if (sizeof(T) == 2 || h.T <= 4) return launch_few<T, 4>(x, w, b, y, p, count, h, s);
+  return launch_few<T, sizeof(T) == 2 ? 4 : 8>(x, w, b, y, p, count, h, s);
+}
+template int launch_few_rows<__half>(const void*, const void*, const void*, const long long*, const Partials<float>&, unsigned*, const Shape&, cudaStream_t);
+template int launch_few_rows<__nv_bfloat16>(const void*, const void*, const void*, const long long*, const Partials<float>&, unsigned*, const Shape&, cudaStream_t);
+template int launch_few_rows<float>(const void*, const void*, const void*, const long long*, const Partials<float>&, unsigned*, const Shape&, cudaStream_t);
+
 // ------------------------------------------------------------------ the tiles of a row joined
 
-// A block has 32 rows; its 32 warps share the slots.  partial: per block the sum of the losses, the rows that count, and
-// whether an ignored row's logits are not finite.
+// A block has 32 rows; its warps share the slots.  partial: per block the sum of the losses, the rows that count, and whether an
+// ignored row's logits are not finite; the last block to finish joins those, in fixed order.
 template <typename A>
 __global__ void __launch_bounds__(1024) combine_kernel(Partials<A> p, const long long* __restrict__ y, int slots, void* loss,
-                                                       A* saved, double* partial, Shape h) {
+                                                       A* saved, double* partial, unsigned* count, Shape h) {
   __shared__ A s_top[32][33], s_sum[32][33], s_all[32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int r = blockIdx.x * 32 + lane;
+  before_all();
   A top = minus_inf<A>(), sum = (A)0, all = (A)0;
   if (r < h.T)
-    for (int s = warp; s < slots; s += 32) {
+    for (int s = warp; s < slots; s += warps) {
       const long long at = (long long)s * h.T + r;
       const A t = p.top[at], n = fmax(top, t), ref = n == minus_inf<A>() ? (A)0 : n;
-      sum = sum * exp2(top - ref) + p.sum[at] * exp2(t - ref);
+      sum = sum * power(top - ref) + p.sum[at] * power(t - ref);
       top = n;
       if (h.smoothing != 0.0) all += p.all[at];
     }
@@ -205,142 +341,64 @@ __global__ void __launch_bounds__(1024) combine_kernel(Partials<A> p, const long
   __syncthreads();
   if (warp) return;
   A most = minus_inf<A>();
-  for (int i = 0; i < 32; ++i) most = fmax(most, s_top[lane][i]);
+#pragma unroll 8
+  for (int i = 0; i < warps; ++i) most = fmax(most, s_top[lane][i]);
   const A ref = most == minus_inf<A>() ? (A)0 : most;
   sum = all = (A)0;
-  for (int i = 0; i < 32; ++i) sum += s_sum[lane][i] * exp2(s_top[lane][i] - ref), all += s_all[lane][i];
-  const A lse2 = ref + log2(sum);
-  double counted = 0, lost = 0, strange = 0;
+#pragma unroll 8
+  for (int i = 0; i < warps; ++i) sum += s_sum[lane][i] * power(s_top[lane][i] - ref), all += s_all[lane][i];
+  const A ls = log(sum);
+  double v[3] = {0, 0, 0};  // loss, rows that count, ignored rows that are not finite
   if (r < h.T) {
     const long long yr = y[r];
-    A v = (A)0;
+    A one = (A)0;
     if (yr != h.ignore) {
-      v = (A)kLn2 * lse2;
-      // a class that does not exist: the loss is NaN (and so are the gradients it reaches)
-      if (yr < 0 || yr >= h.V) v = (A)CUDART_NAN_F;
-      else if (h.smoothing != 1.0) v -= (A)(1.0 - h.smoothing) * p.picked[r];
-      if (h.smoothing != 0.0) v -= (A)(h.smoothing / h.V) * all;
-      counted = 1, lost = (double)v;
+      // from differences to the largest logit: a loss near zero is not that of two large numbers
+      one = ls;
+      if (yr < 0 || yr >= h.V) one = (A)CUDART_NAN_F;  // a class that does not exist: so are the gradients it reaches
+      else if (h.smoothing != 1.0) one += (A)(1.0 - h.smoothing) * (ref - p.picked[r]);
+      if (h.smoothing != 0.0) one += (A)h.smoothing * (ref - all / (A)h.V);
+      v[0] = (double)one, v[1] = 1;
     } else {
-      strange = isfinite(lse2) ? 0 : 1;
+      v[2] = isfinite(ref + ls) ? 0 : 1;
     }
-    if (h.reduction == DK_REDUCE_NONE) ((A*)loss)[r] = v;
-    if (saved) saved[r] = lse2;
+    if (h.reduction == DK_REDUCE_NONE) ((A*)loss)[r] = one;
+    if (saved) saved[r] = ref, saved[h.T + r] = (A)1 / sum;
   }
+  if (!saved && h.reduction == DK_REDUCE_NONE) return;
+  for (int k = 0; k < 3; ++k)
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    counted += __shfl_xor_sync(0xffffffffu, counted, o);
-    lost += __shfl_xor_sync(0xffffffffu, lost, o);
-    strange += __shfl_xor_sync(0xffffffffu, strange, o);
+    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if (gridDim.x > 1) {
+    unsigned turn = 0;
+    if (lane == 0) {
+      for (int k = 0; k < 3; ++k) partial[3 * blockIdx.x + k] = v[k];
+      __threadfence();
+      turn = atomicAdd(count, 1u);
+    }
+    if (__shfl_sync(0xffffffffu, turn, 0) != gridDim.x - 1) return;
+    __threadfence();
+    v[0] = v[1] = v[2] = 0;
+    for (unsigned i = lane; i < gridDim.x; i += 32)
+      for (int k = 0; k < 3; ++k) v[k] += __ldcg(partial + 3 * i + k);
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
   }
   if (lane) return;
-  if (gridDim.x > 1) {
-    partial[3 * blockIdx.x] = lost, partial[3 * blockIdx.x + 1] = counted, partial[3 * blockIdx.x + 2] = strange;
-  } else {
-    if (h.reduction != DK_REDUCE_NONE) *(A*)loss = (A)(h.reduction == DK_REDUCE_MEAN ? lost / counted : lost);
-    if (saved) saved[h.T] = (A)counted, saved[h.T + 1] = (A)strange;
-  }
-}
-
-// the blocks of combine_kernel joined, in fixed order
-template <typename A>
-__global__ void __launch_bounds__(1024) finish_kernel(const double* __restrict__ partial, int blocks, void* loss, A* saved, Shape h) {
-  __shared__ double s[3][32];
-  double v[3] = {0, 0, 0};
-  for (int i = threadIdx.x; i < blocks; i += 1024)
-    for (int k = 0; k < 3; ++k) v[k] += partial[3 * i + k];
-  for (int k = 0; k < 3; ++k) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-    if ((threadIdx.x & 31) == 0) s[k][threadIdx.x >> 5] = v[k];
-  }
-  __syncthreads();
-  if (threadIdx.x >= 32) return;
-  for (int k = 0; k < 3; ++k) {
-    v[k] = s[k][threadIdx.x];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-  }
-  if (threadIdx.x) return;
   if (h.reduction != DK_REDUCE_NONE) *(A*)loss = (A)(h.reduction == DK_REDUCE_MEAN ? v[0] / v[1] : v[0]);
-  if (saved) saved[h.T] = (A)v[1], saved[h.T + 1] = (A)v[2];
-}
-
-// ------------------------------------------------------------------ what arrives for each row
-
-// for a whole call, g of a row that counts (not DK_REDUCE_NONE)
-template <typename A>
-__device__ __forceinline__ A common_g(const A* up, const A* saved, const Shape& h) {
-  return h.reduction == DK_REDUCE_MEAN ? up[0] / saved[h.T] : up[0];
-}
-// the power of two that brings `largest` to [2^14, 2^15)
-template <typename A>
-__device__ __forceinline__ A scale_for(A largest) {
-  if (!(largest > (A)0) || !isfinite(largest)) return (A)1;
-  const int e = 14 - ilogb(largest);
-  return (A)ldexp(1.0, e < -100 ? -100 : e > 100 ? 100 : e);
-}
-
-// the largest |g| of the rows, one block
-template <typename A>
-__global__ void __launch_bounds__(1024) largest_kernel(const A* __restrict__ up, const long long* __restrict__ y, A* back, Shape h) {
-  __shared__ A s[32];
-  A v = (A)0;
-  for (int r = threadIdx.x; r < h.T; r += 1024)
-    if (y[r] != h.ignore) v = fmax(v, fabs(up[r]));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  if (threadIdx.x >= 32) return;
-  v = s[threadIdx.x];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if (threadIdx.x == 0) back[1] = v;
-}
-
-// g_t: what arrives for row t; nothing for an ignored one, NaN for a class that does not exist
-template <typename A>
-__global__ void rows_kernel(const A* __restrict__ up, const long long* __restrict__ y, const A* __restrict__ saved, A* __restrict__ g,
-                            A* back, Shape h) {
-  const int r = blockIdx.x * blockDim.x + threadIdx.x;
-  if (r >= h.T) return;
-  const long long yr = y[r];
-  const bool each = h.reduction == DK_REDUCE_NONE;
-  A v = each ? up[r] : common_g(up, saved, h);
-  if (back) {
-    const A f = scale_for(each ? back[1] : (A)fabs(v));
-    if (r == 0) back[0] = (A)1 / f;
-    v *= f;
-  }
-  if (yr == h.ignore) v = (A)0;
-  else if (yr < 0 || yr >= h.V) v = (A)CUDART_NAN_F;
-  g[r] = v;
+  if (saved) saved[2ll * h.T] = (A)v[1], saved[2ll * h.T + 1] = (A)v[2];
 }
 
 template <typename A>
 int launch_combine(const Partials<A>& p, const long long* y, int slots, void* loss, void* saved, double* partial, const Shape& h,
                    cudaStream_t s) {
-  const int blocks = div_up(h.T, kCombineRows);
-  combine_kernel<A><<<blocks, 1024, 0, s>>>(p, y, slots, loss, (A*)saved, partial, h);
-  const int rc = check_launch();
-  if (rc != DK_OK || blocks == 1) return rc;
-  finish_kernel<A><<<1, 1024, 0, s>>>(partial, blocks, loss, (A*)saved, h);
-  return check_launch();
+  int warps = 1;  // four slots a warp
+  while (warps < 32 && warps * 4 < slots) warps *= 2;
+  return launch_after(combine_kernel<A>, div_up(h.T, kCombineRows), 32 * warps, 0, 1, s, p, y, slots, loss, (A*)saved, partial,
+                      combine_count(partial, h.T), h);
 }
 template int launch_combine<float>(const Partials<float>&, const long long*, int, void*, void*, double*, const Shape&, cudaStream_t);
-
-template <typename A>
-int launch_rows(const void* up, const long long* y, const void* saved, A* g, A* back, const Shape& h, cudaStream_t s) {
-  if (back && h.reduction == DK_REDUCE_NONE) {
-    largest_kernel<A><<<1, 1024, 0, s>>>((const A*)up, y, back, h);
-    const int rc = check_launch();
-    if (rc != DK_OK) return rc;
-  }
-  rows_kernel<A><<<div_up(h.T, 256), 256, 0, s>>>((const A*)up, y, (const A*)saved, g, back, h);
-  return check_launch();
-}
-template int launch_rows<float>(const void*, const long long*, const void*, float*, float*, const Shape&, cudaStream_t);
 
 // ------------------------------------------------------------------ fp64 calls
 
@@ -363,7 +421,7 @@ ForwardPlan forward_plan(int T, int V) {
 
 struct BackwardPlan {
   int vc;  // classes of a piece
-  size_t g, dz, bytes;
+  size_t dz, bytes;
 };
 BackwardPlan backward_plan(int T, int V) {
   BackwardPlan p;
@@ -371,7 +429,7 @@ BackwardPlan backward_plan(int T, int V) {
   long long vc = (64ll << 20) / ((long long)T * 8) / kTile * kTile;
   if (vc < kTile) vc = kTile;
   p.vc = vc < V ? (int)vc : V;
-  p.g = l.take((size_t)T * 8), p.dz = l.take((size_t)T * p.vc * 8);
+  p.dz = l.take((size_t)T * p.vc * 8);
   p.bytes = l.bytes;
   return p;
 }
@@ -384,9 +442,10 @@ int forward64(const double* x, const double* w, const double* b, const long long
   if (row_tiles > 65535) return DK_ERR_UNSUPPORTED;
   char* m = (char*)ws;
   const Partials<double> part = {(double*)(m + p.top), (double*)(m + p.sum), (double*)(m + p.all), (double*)(m + p.picked)};
-  logits_stats_kernel<<<dim3(p.slots, row_tiles), 256, 0, s>>>(x, w, b, y, part, h);
+  double* partial = (double*)(m + p.partial);
+  logits_stats_kernel<<<dim3(p.slots, row_tiles), 256, 0, s>>>(x, w, b, y, part, combine_count(partial, h.T), h);
   const int rc = check_launch();
-  return rc != DK_OK ? rc : launch_combine<double>(part, y, p.slots, loss, saved, (double*)(m + p.partial), h, s);
+  return rc != DK_OK ? rc : launch_combine<double>(part, y, p.slots, loss, saved, partial, h, s);
 }
 
 int backward64(const void* up, const double* x, const double* w, const double* b, const long long* y, const double* saved, double* dx,
@@ -395,11 +454,12 @@ int backward64(const void* up, const double* x, const double* w, const double* b
   if (!ws || ws_bytes < p.bytes) return DK_ERR_WORKSPACE;
   const int row_tiles = div_up(h.T, kTile), feature_tiles = div_up(h.D, kTile);
   if (row_tiles > 65535 || div_up(p.vc, kTile) > 65535) return DK_ERR_UNSUPPORTED;
-  double *g = (double*)((char*)ws + p.g), *dz = (double*)((char*)ws + p.dz);
-  int rc = launch_rows<double>(up, y, saved, g, nullptr, h, s);
+  double* dz = (double*)((char*)ws + p.dz);
+  const Upstream<double> u = {(const double*)up, saved + 2ll * h.T, nullptr, h.reduction, 1.0};
+  int rc = DK_OK;
   for (int v0 = 0; v0 < h.V && rc == DK_OK; v0 += p.vc) {
     const int vc = h.V - v0 < p.vc ? h.V - v0 : p.vc, class_tiles = div_up(vc, kTile);
-    logits_dz_kernel<<<dim3(class_tiles, row_tiles), 256, 0, s>>>(x, w, b, y, saved, g, dz, v0, vc, h);
+    logits_dz_kernel<<<dim3(class_tiles, row_tiles), 256, 0, s>>>(x, w, b, y, saved, u, dz, v0, vc, h);
     rc = check_launch();
     if (rc == DK_OK && dx) {
       product_kernel<<<dim3(feature_tiles, row_tiles), 256, 0, s>>>(dz, vc, 1, w + (long long)v0 * h.D, nullptr, 0, dx, h.T, h.D, vc, v0 == 0);

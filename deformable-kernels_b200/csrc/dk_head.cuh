@@ -21,8 +21,8 @@ struct Shape {
 // What a tile of logits leaves of its rows; a slot is a run of classes.
 template <typename A>
 struct Partials {
-  A* top;     // [slots][T] maximum of z log2(e)
-  A* sum;     // [slots][T] sum of 2^(z log2(e) - top)
+  A* top;     // [slots][T] maximum of z
+  A* sum;     // [slots][T] sum of exp(z - top): the largest logit's term is exactly one
   A* all;     // [slots][T] sum of z (label smoothing only)
   A* picked;  // [T] z of the row's own class
 };
@@ -40,17 +40,74 @@ struct Layout {
   }
 };
 
-// ---- small kernels (dk_head.cu)
-constexpr int kCombineRows = 32;  // rows of a block of the kernel that joins the slots
-inline size_t combine_bytes(int T) { return (size_t)div_up(T, kCombineRows) * 3 * sizeof(double); }
-// losses, log-sum-exps and counts from the slots; `partial`: combine_bytes()
+// What arrives from behind the loss, g_t.  dz_t = g_t (p - (1 - s) [v = y_t] - s / V) is an operand of two products, so the factor that all
+// its rows have in common is left to their results: what is rounded to 16 bits is dz `unit` / g, with `unit` 1 / (1 - s) so that a class that the
+// network gives no chance has exactly one (a power of two): the rounding of g (1 - s) would be the same in every row and add up.  fp16: `unit`
+// has a factor 2^14 besides, which keeps small probabilities out of the subnormal numbers.  DK_REDUCE_NONE: every row has its own g; `unit`
+// brings the largest to [2^14, 2^15) (fp16) or is 1.
+template <typename A>
+struct Upstream {
+  const A* up;       // one value, or one a row (DK_REDUCE_NONE)
+  const A* count;    // rows that count
+  const A* largest;  // DK_REDUCE_NONE, fp16: the largest |up| of those
+  int reduction;
+  A unit;
+};
+template <typename A>
+__device__ __forceinline__ A upstream_unit(const Upstream<A>& u) {
+  if (!u.largest) return u.unit;
+  const A largest = *u.largest;
+  if (!(largest > (A)0) || !isfinite(largest)) return (A)1;
+  const int e = 14 - ilogb(largest);
+  return (A)ldexp((A)1, e < -100 ? -100 : e > 100 ? 100 : e);
+}
+// dz's factor of row r, whose class is y: nothing for an ignored row, NaN for a class that does not exist
+template <typename A>
+__device__ __forceinline__ A upstream_row(const Upstream<A>& u, int r, long long y, long long ignore, int classes) {
+  if (y == ignore) return (A)0;
+  if (y < 0 || y >= classes) return (A)(0.0 / 0.0);
+  return u.reduction == DK_REDUCE_NONE ? u.up[r] * upstream_unit(u) : u.unit;
+}
+// the factor of the products
+template <typename A>
+__device__ __forceinline__ A upstream_back(const Upstream<A>& u) {
+  if (u.reduction == DK_REDUCE_NONE) return (A)1 / upstream_unit(u);
+  if (*u.count == (A)0) return (A)0;  // no row counts: their dz are zeros, and the mean's g is not finite
+  return (u.reduction == DK_REDUCE_MEAN ? u.up[0] / *u.count : u.up[0]) / u.unit;
+}
+
+// ---- the slots of a row joined (dk_head.cu)
+constexpr int kCombineRows = 32;  // rows of a block
+// sums of the blocks, and the count of those that are done, which the kernel before sets to zero
+inline size_t combine_bytes(int T) { return (size_t)div_up(T, kCombineRows) * 3 * sizeof(double) + sizeof(double); }
+// losses, log-sum-exps and counts; `partial`: combine_bytes(), the count last
 template <typename A>
 int launch_combine(const Partials<A>& p, const long long* y, int slots, void* loss, void* saved, double* partial, const Shape& h,
                    cudaStream_t s);
-// g_t of every row.  `back` (NULL: nothing is scaled): two floats, g comes out multiplied with a power of two that brings the
-// largest to about 2^14, back[0] is the reciprocal of that
-template <typename A>
-int launch_rows(const void* up, const long long* y, const void* saved, A* g, A* back, const Shape& h, cudaStream_t s);
+inline unsigned* combine_count(double* partial, int T) { return (unsigned*)(partial + 3ll * div_up(T, kCombineRows)); }
+
+// ---- the loss of a few rows (dk_head.cu): memory is the bound, the products are taken on the CUDA cores
+bool few_rows(int T, int dtype);
+int few_slots(int V);
+template <typename T>
+int launch_few_rows(const void* x, const void* w, const void* b, const long long* y, const Partials<float>& p, unsigned* count,
+                    const Shape& h, cudaStream_t s);
+
+// ---- launches that may begin while the kernel before still runs: before_all() waits for what it wrote
+__device__ __forceinline__ void before_all() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+template <typename K, typename... Args>
+int launch_after(K kernel, unsigned grid, unsigned block, size_t smem, int cluster, cudaStream_t s, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid), cfg.blockDim = dim3(block), cfg.dynamicSmemBytes = smem, cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
+  return check_launch();
+}
 
 // ---- fp16, bf16 and fp32 on the tensor cores (dk_head_tc.cu)
 size_t tc_forward_bytes(int T, int D, int V, int dtype);

@@ -8,8 +8,9 @@
 // tile.  An operand is K-major (rows of the tensor are rows of the product) or MN-major (columns are); both
 // come as boxes of 64 x 64 values, 128 swizzled bytes a row.
 //
-// fp32 operands are three bf16 pieces each (8 bits a piece, 24 in all); the six products of pieces that reach 2^-24 are summed
-// in the same accumulator, the smallest first, so that the additions that cut are those of small sums.
+// fp32 operands are three bf16 pieces each (8 bits a piece, 24 in all).  A stage holds one piece of both; the six products of
+// pieces that reach 2^-24 are taken from three stages, that of the leading pieces into one accumulator, the five
+// small ones into another: the additions of the tensor cores cut, and a cut of the small sum costs nothing.
 #include <math_constants.h>
 
 #include <type_traits>
@@ -205,6 +206,8 @@ template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(unsigned v) 
 
 // ---- arguments
 
+__device__ __forceinline__ int div_up_device(int a, int b) { return (a + b - 1) / b; }
+
 enum Role { kStats, kDz, kGrad };
 
 // one of the gradient products, out[M][N] = sum over K; tiles [splits][m][n]
@@ -214,6 +217,11 @@ struct Product {
   float* acc;                 // running sum over the pieces, or [splits][M][N]
   void* out;                  // NULL: the sums stay in acc
   int first;                  // 0: add what acc holds
+};
+
+// which items a cluster takes (item_of); short_less <= short_more
+struct Schedule {
+  int long_product, n_long, n_short, short_less, short_more;
 };
 
 struct Args {
@@ -230,14 +238,24 @@ struct Args {
   float* sum;
   float* all;                 // NULL without label smoothing
   float* picked;
-  const float* lse2;
-  const float* g;
+  unsigned* done;             // forward: set to zero for the kernel that follows
+  const float *ref, *inv;     // of the piece's rows: p = exp(z - ref) inv
+  Upstream<float> up;
+  int all_classes;            // of the call
   float* column_sums;         // [rows / 32][classes], NULL: no bias gradient
   float smooth_each, smooth_own;  // s / V, 1 - s
+  const float* strange;       // != 0: some ignored row's features are not finite, x_clean has them zeroed; NULL: they are zero anyway
+  const void* dirty;          // backward, first piece: x, of which `clean` becomes a copy without ignored rows where `strange` says so
+  void* clean;
+  int width;                  // of x
+  int up_rows;                // of the call
+  const long long* target_all;
   // gradients
   Product dw, dx;
-  const float* strange;       // != 0: some ignored row's features are not finite, x_clean has them zeroed
-  const float* back;          // what the gradients are multiplied with (fp16: dz is scaled); NULL: nothing
+  Schedule schedule;
+  float* acc_b;               // bias gradient of the pieces before
+  void* out_b;                // NULL: it goes to acc_b
+  int first_b;
 };
 
 struct Item {
@@ -246,31 +264,105 @@ struct Item {
   int split, first, count;  // steps of K
 };
 
+// The i-th item of a cluster.  The tiles of the logits are alike and go round.  Those of the two gradient products are not: the product with
+// the longer sums goes round first, and of the shorter ones the clusters that got one less of the long get `short_more` rounds, the
+// others `short_less` (Schedule below), so that all end together.
 template <int ROLE>
-__device__ __forceinline__ int items_of(const Args& a) {
-  if (ROLE != kGrad) return a.tiles_m * a.tiles_n;
-  return a.dw.tiles_m * a.dw.tiles_n * a.dw.splits + a.dx.tiles_m * a.dx.tiles_n * a.dx.splits;
-}
-template <int ROLE>
-__device__ __forceinline__ Item item_of(const Args& a, int i) {
-  Item t;
+__device__ __forceinline__ bool item_of(const Args& a, int cluster, int clusters, int i, Item& t) {
   t.product = 0, t.split = 0, t.first = 0, t.count = a.depth;
   if (ROLE != kGrad) {
+    i = i * clusters + cluster;
+    if (i >= a.tiles_m * a.tiles_n) return false;
     // columns of tiles, `group` tiles of rows high: their part of x stays in L2 while the weights stream past once a group
     const int per = a.group * a.tiles_n, gi = i / per, left = a.tiles_m - gi * a.group, high = left < a.group ? left : a.group;
     const int r = i - gi * per;
     t.n = r / high, t.m = gi * a.group + r - t.n * high;
-    return t;
+    return true;
   }
-  const int own = a.dw.tiles_m * a.dw.tiles_n * a.dw.splits;
-  t.product = i >= own;
+  const Schedule& c = a.schedule;
+  const int rest = c.n_long % clusters;
+  const bool more_long = cluster < rest;
+  const int own_long = c.n_long / clusters + (more_long ? 1 : 0);
+  bool is_long = i < own_long;
+  if (is_long) {
+    i = i * clusters + cluster;
+  } else {
+    i -= own_long;
+    const int own_short = more_long ? c.short_less : c.short_more;
+    if (i >= own_short) return false;
+    // rounds of all clusters, then those of the clusters with more of them
+    i = i < c.short_less ? i * clusters + cluster : c.short_less * clusters + (i - c.short_less) * (clusters - rest) + cluster - rest;
+    if (i >= c.n_short) return false;
+  }
+  t.product = is_long ? c.long_product : 1 - c.long_product;
   const Product& p = t.product ? a.dx : a.dw;
-  if (t.product) i -= own;
   t.n = i % p.tiles_n, i /= p.tiles_n;
   t.m = i % p.tiles_m, t.split = i / p.tiles_m;
   t.first = t.split * p.per;
   t.count = p.blocks - t.first < p.per ? p.blocks - t.first : p.per;
-  return t;
+  return true;
+}
+
+// ---- on the side, a warp of every block
+
+// the 16-bit x with its ignored rows zeroed
+__device__ __forceinline__ void clean_rows(const Args& a, int lane) {
+  const int pieces = a.width / 8;
+  const uint4* src = (const uint4*)a.dirty;
+  uint4* dst = (uint4*)a.clean;
+  for (int r = blockIdx.x; r < a.up_rows; r += gridDim.x) {
+    const bool in = a.target_all[r] != a.ignore;
+    for (int q = lane; q < pieces; q += 32) dst[(long long)r * pieces + q] = in ? src[(long long)r * pieces + q] : make_uint4(0, 0, 0, 0);
+  }
+}
+
+// db from the sums over 32 rows each, in fixed order: a warp has 32 classes, or fewer (and several lanes for each) where that keeps
+// more warps busy
+template <typename O>
+__device__ __forceinline__ void join_columns(const Args& a, int lane) {
+  int wide = 32;
+  while (wide > 4 && div_up_device(a.classes, wide) * 2 <= (int)gridDim.x) wide >>= 1;
+  const int slabs = div_up_device(a.rows, 32), c_lane = lane & (wide - 1), s_lane = lane / wide, step = 32 / wide;
+  const float back = upstream_back(a.up);
+  for (int c0 = blockIdx.x * wide; c0 < a.classes; c0 += gridDim.x * wide) {
+    const int c = c0 + c_lane;
+    float v = 0;
+    if (c < a.classes) {
+#pragma unroll 8
+      for (int r = s_lane; r < slabs; r += step) v += a.column_sums[(long long)r * a.classes + c];
+    }
+    for (int o = wide; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (s_lane == 0 && c < a.classes) {
+      v *= back;
+      if (!a.first_b) v += a.acc_b[c];
+      if (a.out_b) ((O*)a.out_b)[c] = (O)v;
+      else a.acc_b[c] = v;
+    }
+  }
+}
+
+// one 64-deep step of a product: four mma; `fresh`: what the accumulator held is dropped
+template <int CG>
+__device__ __forceinline__ void product(unsigned d, uint64_t a, uint64_t b, unsigned at, unsigned idesc, unsigned step_a, unsigned step_b,
+                                        bool fresh) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) mma_ss<CG>(d + at, a + (uint64_t)(q * step_a >> 4), b + (uint64_t)(q * step_b >> 4), idesc, !fresh || q > 0);
+}
+
+// 32 columns of the finished accumulator
+template <int BN, int PIECES>
+__device__ __forceinline__ void take(float (&v)[32], unsigned a) {
+  ld32(v, a);
+  if (PIECES == 1) {
+    wait_ld(v);
+  } else {
+    float small[32];
+    ld32(small, a + BN);
+    wait_ld(v);
+    wait_ld(small);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += small[j];
+  }
 }
 
 // ---- the kernel
@@ -282,7 +374,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
   constexpr int kBoxesB = BN / CG / kBox;          // boxes of B a block loads
   constexpr int kGroups = BN >= 128 ? 2 : 1;       // epilogue warps side by side
   constexpr int kWide = BN / kGroups;              // columns of an epilogue warp
-  constexpr int kPairs = PIECES == 1 ? 1 : 6;
+  constexpr int kAcc = PIECES == 1 ? BN : 2 * BN;  // columns of an accumulator
+  static_assert(2 * kAcc <= 512, "two accumulators in TMEM");
   SharedTail& t = *reinterpret_cast<SharedTail*>(smem + kStages * kStage + 8 * kStageWarp);
   const unsigned base = smem_u32(smem);
   if (base & 1023) {  // the swizzled boxes need it; the same in every block
@@ -292,7 +385,6 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned rank = CG == 1 ? 0u : cluster_rank();
   const int cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
-  const int items = items_of<ROLE>(a);
   volatile int* abort_flag = &t.abort_flag;
 
   if (threadIdx.x == 0) {
@@ -308,19 +400,19 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
   tc::fence_after();
   const unsigned tmem = t.tmem;
 
+  let_next();
   if (warp == 0) {
     // ---------------- producer
     const bool one = tc::elect_one();
     const CUtensorMap* mx = &a.x;
+    before_all();
     if (ROLE == kGrad && a.strange && *a.strange != 0.0f) mx = &a.x_clean;
     int fill = 0;
-    for (int i = cluster; i < items; i += clusters) {
-      const Item it = item_of<ROLE>(a, i);
+    Item it;
+    for (int i = 0; item_of<ROLE>(a, cluster, clusters, i, it); ++i) {
       const int m0 = (it.m * CG + (int)rank) * 128, n0 = it.n * BN + (int)rank * (BN / CG);
-      for (int pr = 0; pr < kPairs; ++pr) {
-        // smallest first: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
-        const int pa = PIECES == 1 ? 0 : (0x001012 >> (4 * pr)) & 15, pb = PIECES == 1 ? 0 : (0x010210 >> (4 * pr)) & 15;
-        for (int kb = it.first; kb < it.first + it.count; ++kb, ++fill) {
+      for (int kb = it.first; kb < it.first + it.count; ++kb) {
+        for (int piece = 0; piece < PIECES; ++piece, ++fill) {
           const int s = fill % kStages;
           if (wait(smem_u32(&t.empty[s]), ((fill / kStages) & 1) ^ 1, abort_flag)) continue;
           const unsigned sa = base + s * kStage, sb = sa + 128 * 128;
@@ -330,14 +422,14 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
             if (rank == 0) ring::mbar_arrive_expect_tx(smem_u32(&t.full[s]), CG * kStage);
             const int k0 = kb * kBox;
             if (ROLE != kGrad) {
-              for (int q = 0; q < 2; ++q) load_box<CG>(sa + q * kBoxBytes, &a.x, k0, a.row0 + m0 + q * kBox, pa, bar);
-              for (int q = 0; q < kBoxesB; ++q) load_box<CG>(sb + q * kBoxBytes, &a.w, k0, a.class0 + n0 + q * kBox, pb, bar);
+              for (int q = 0; q < 2; ++q) load_box<CG>(sa + q * kBoxBytes, &a.x, k0, a.row0 + m0 + q * kBox, piece, bar);
+              for (int q = 0; q < kBoxesB; ++q) load_box<CG>(sb + q * kBoxBytes, &a.w, k0, a.class0 + n0 + q * kBox, piece, bar);
             } else if (it.product == 0) {
-              for (int q = 0; q < 2; ++q) load_box<CG>(sa + q * kBoxBytes, &a.dz, m0 + q * kBox, k0, pa, bar);
-              for (int q = 0; q < kBoxesB; ++q) load_box<CG>(sb + q * kBoxBytes, mx, n0 + q * kBox, a.row0 + k0, pb, bar);
+              for (int q = 0; q < 2; ++q) load_box<CG>(sa + q * kBoxBytes, &a.dz, m0 + q * kBox, k0, piece, bar);
+              for (int q = 0; q < kBoxesB; ++q) load_box<CG>(sb + q * kBoxBytes, mx, n0 + q * kBox, a.row0 + k0, piece, bar);
             } else {
-              for (int q = 0; q < 2; ++q) load_box<CG>(sa + q * kBoxBytes, &a.dz, k0, m0 + q * kBox, pa, bar);
-              for (int q = 0; q < kBoxesB; ++q) load_box<CG>(sb + q * kBoxBytes, &a.w, n0 + q * kBox, a.class0 + k0, pb, bar);
+              for (int q = 0; q < 2; ++q) load_box<CG>(sa + q * kBoxBytes, &a.dz, k0, m0 + q * kBox, piece, bar);
+              for (int q = 0; q < kBoxesB; ++q) load_box<CG>(sb + q * kBoxBytes, &a.w, n0 + q * kBox, a.class0 + k0, piece, bar);
             }
           }
           __syncwarp();
@@ -355,8 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
       const bool one = tc::elect_one();
       constexpr unsigned kDesc = (1u << 4) | type_bits<E>() | ((unsigned)(BN >> 3) << 17) | ((unsigned)(128 * CG >> 4) << 24);
       int fill = 0, tile = 0;
-      for (int i = cluster; i < items; i += clusters, ++tile) {
-        const Item it = item_of<ROLE>(a, i);
+      Item it;
+      for (; item_of<ROLE>(a, cluster, clusters, tile, it); ++tile) {
         // both operands of the logits are K-major; W and x of the gradients are MN-major, dz is either
         const bool ta = ROLE == kGrad && it.product == 0, tb = ROLE == kGrad;
         const unsigned idesc = kDesc | ((unsigned)ta << 15) | ((unsigned)tb << 16);
@@ -364,19 +456,31 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         const int b = tile & 1;
         bool gone = wait(smem_u32(&t.acc_empty[b]), ((tile >> 1) & 1) ^ 1, abort_flag);
         tc::fence_after();
-        const unsigned d = tmem + b * BN;
-        const int steps = it.count * kPairs;
-        for (int k = 0; k < steps; ++k, ++fill) {
-          const int s = fill % kStages;
-          gone = wait(smem_u32(&t.full[s]), (fill / kStages) & 1, abort_flag);
+        const unsigned d = tmem + b * kAcc;
+        for (int k = 0; k < it.count; ++k, fill += PIECES) {
+          uint64_t da[PIECES], db[PIECES];
+#pragma unroll
+          for (int p = 0; p < PIECES; ++p) {
+            const int s = (fill + p) % kStages;
+            gone = wait(smem_u32(&t.full[s]), ((fill + p) / kStages) & 1, abort_flag);
+            if (gone) break;
+            tc::fence_after();
+            const unsigned sa = base + s * kStage;
+            da[p] = swizzled(sa, lead, 1024), db[p] = swizzled(sa + 128 * 128, lead, 1024);
+            if (one) {
+              // product (i, j) of pieces i + j <= 2 as soon as the later of the two has landed
+#pragma unroll
+              for (int i = 0; i <= p; ++i) {
+                if (PIECES == 1 || i + p <= 2) product<CG>(d, da[p], db[i], p == 0 ? 0 : BN, idesc, step_a, step_b, k == 0 && (p == 0 || (p == 1 && i == 0)));
+                if (i != p && i + p <= 2) product<CG>(d, da[i], db[p], BN, idesc, step_a, step_b, false);
+              }
+            }
+            __syncwarp();
+          }
           if (gone) continue;
-          tc::fence_after();
-          const unsigned sa = base + s * kStage, sb = sa + 128 * 128;
-          const uint64_t da = swizzled(sa, lead, 1024), db = swizzled(sb, lead, 1024);
           if (one) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) mma_ss<CG>(d, da + (uint64_t)(q * step_a >> 4), db + (uint64_t)(q * step_b >> 4), idesc, k > 0 || q > 0);
-            commit<CG>(smem_u32(&t.empty[s]));
+            for (int p = 0; p < PIECES; ++p) commit<CG>(smem_u32(&t.empty[(fill + p) % kStages]));
           }
           __syncwarp();
         }
@@ -384,21 +488,28 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         __syncwarp();
       }
     }
+  } else if (warp == 3) {
+    // ---------------- what else there is to do
+    before_all();
+    if (ROLE == kStats && blockIdx.x == 0 && lane == 0) *a.done = 0;
+    if (ROLE == kDz && a.clean && *a.strange != 0.0f) clean_rows(a, lane);
+    if (ROLE == kGrad && a.column_sums) join_columns<typename std::conditional<PIECES == 1, E, float>::type>(a, lane);
   } else if (warp >= 4 && (warp - 4) >> 2 < kGroups) {
     // ---------------- epilogue
+    before_all();
     const int sub = warp & 3, grp = (warp - 4) >> 2;
     const unsigned stage = base + kStages * kStage + (warp - 4) * kStageWarp;
     const unsigned lanes = (unsigned)(32 * sub) << 16;
     constexpr float kL2 = (float)kLog2e;
     int tile = 0;
-    for (int i = cluster; i < items; i += clusters, ++tile) {
-      const Item it = item_of<ROLE>(a, i);
+    Item it;
+    for (; item_of<ROLE>(a, cluster, clusters, tile, it); ++tile) {
       const int b = tile & 1;
       const int row_base = (it.m * CG + (int)rank) * 128 + 32 * sub, row = row_base + lane;
       const int col_base = it.n * BN + grp * kWide;
       float* bias = t.bias[b];
       long long y = -1;
-      float l2 = 0, g = 0;
+      float ref = 0, inv = 0, g = 0;
       bool live = false;
       if (ROLE != kGrad) {
         // what is added to the logits; -inf outside, where the product is zero
@@ -409,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         }
         if (row < a.rows) {
           y = a.target[row];
-          if (ROLE == kDz) l2 = a.lse2[row], g = a.g[row], live = y != a.ignore;
+          if (ROLE == kDz) ref = a.ref[row], inv = a.inv[row], g = upstream_row(a.up, row, y, a.ignore, a.all_classes), live = y != a.ignore;
         }
         __syncwarp();
         asm volatile("bar.sync 1, %0;\n" ::"n"(128 * kGroups) : "memory");
@@ -419,15 +530,14 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
       const int own = far >= 0 && far < kWide ? (int)far : -1;
       (void)wait(smem_u32(&t.acc_full[b]), (tile >> 1) & 1, abort_flag);
       tc::fence_after();
-      const unsigned d = tmem + lanes + b * BN + grp * kWide;
+      const unsigned d = tmem + lanes + b * kAcc + grp * kWide;
       if (ROLE == kStats) {
         float top = -CUDART_INF_F, sum = 0, all = 0, picked = 0;
 #pragma unroll 1
         for (int c0 = 0; c0 < kWide; c0 += 32) {
           float z[32];
           __syncwarp();
-          ld32(z, d + c0);
-          wait_ld(z);
+          take<BN, PIECES>(z, d + c0);
           const float4* bp = reinterpret_cast<const float4*>(bias + grp * kWide + c0);
           float most = -CUDART_INF_F;
 #pragma unroll
@@ -447,11 +557,11 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           }
 #pragma unroll
           for (int j = 0; j < 32; ++j) most = fmaxf(most, z[j]);
-          const float n = fmaxf(top, most * kL2), ref = n == -CUDART_INF_F ? 0.0f : n;
-          float part = 0;
+          const float n = fmaxf(top, most), ref = n == -CUDART_INF_F ? 0.0f : n;
+          float part[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) part += ex2(fmaf(z[j], kL2, -ref));
-          sum = sum * ex2(top - ref) + part;
+          for (int j = 0; j < 32; ++j) part[j & 3] += ex2((z[j] - ref) * kL2);
+          sum = sum * ex2((top - ref) * kL2) + ((part[0] + part[1]) + (part[2] + part[3]));
           top = n;
         }
         if (row < a.rows) {
@@ -467,10 +577,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           if (!inside) break;  // of the whole warp
           float v[2][32];
           __syncwarp();
-          ld32(v[0], d + c0);
-          ld32(v[1], d + c0 + 32);
-          wait_ld(v[0]);
-          wait_ld(v[1]);
+          take<BN, PIECES>(v[0], d + c0);
+          take<BN, PIECES>(v[1], d + c0 + 32);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float4* bp = reinterpret_cast<const float4*>(bias + grp * kWide + c0 + 32 * h);
@@ -481,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
             }
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-              float p = ex2(fmaf(v[h][j], kL2, -l2)) - a.smooth_each;
+              float p = fmaf(ex2((v[h][j] - ref) * kL2), inv, -a.smooth_each);
               if (own == c0 + 32 * h + j) p -= a.smooth_own;
               v[h][j] = live ? p * g : 0.0f;
             }
@@ -527,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         }
       } else {
         const Product& p = it.product ? a.dx : a.dw;
-        const float back = a.back ? *a.back : 1.0f;
+        const float back = upstream_back(a.up);
         float* acc = p.acc ? p.acc + (p.splits > 1 ? (long long)it.split * p.M * p.N : 0) : nullptr;
         const bool out16 = PIECES == 1 && p.out;  // 16-bit results; else fp32, to the gradient or to the sums
         float* to32 = p.out ? (float*)p.out : acc;
@@ -537,8 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           if (row_base >= p.M || col_base + c0 >= p.N) break;  // of the whole warp
           float v[32];
           __syncwarp();
-          ld32(v, d + c0);
-          wait_ld(v);
+          take<BN, PIECES>(v, d + c0);
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             sts16(staged(stage, lane, q), __float_as_uint(v[4 * q] * back), __float_as_uint(v[4 * q + 1] * back),
@@ -604,45 +711,78 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
 
 template <typename T> __device__ __forceinline__ float as_float(T v) { return (float)v; }
 
-// [rows][width] -> PIECES planes [rows][pitch] of E: fp32 in three bf16 pieces, 16-bit rows on 16 bytes.  target (NULL: all
-// rows count): rows whose target is `ignore` become zeros.
+struct LayOut {
+  const void* src;
+  void* dst;
+  long long groups;          // of eight values of a row
+  int width, per_row;        // per_row: groups of a row
+  long long plane;           // values of a plane
+  const long long* target;   // rows whose target is `ignore` become zeros; NULL: all rows count
+};
+// [rows][width] -> PIECES planes [rows][8 per_row] of E: fp32 in three bf16 pieces, 16-bit rows on 16 bytes; eight values a thread
 template <typename T, typename E, int PIECES>
-__global__ void __launch_bounds__(256) lay_out_kernel(const T* __restrict__ src, E* __restrict__ dst, int rows, int width, int pitch,
-                                                      const long long* __restrict__ target, long long ignore) {
-  const long long total = (long long)rows * pitch, plane = total;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const int r = (int)(i / pitch), c = (int)(i - (long long)r * pitch);
-    const bool in = c < width && !(target && target[r] == ignore);
-    const T v = in ? src[(long long)r * width + c] : (T)0.0f;
+__device__ __forceinline__ void lay_out_group(const LayOut& l, long long i, long long ignore) {
+  const long long r = l.groups < 0x7fffffff ? (long long)((unsigned)i / (unsigned)l.per_row) : i / l.per_row;
+  const int c = (int)(i - r * l.per_row) * 8;
+  const T* src = (const T*)l.src + r * l.width + c;
+  const bool in = !(l.target && l.target[r] == ignore);
+  T v[8];
+  if (in && l.width % 8 == 0) {
+    constexpr int kVec = 8 * sizeof(T) / 16;
+#pragma unroll
+    for (int q = 0; q < kVec; ++q) reinterpret_cast<uint4*>(v)[q] = __ldg(reinterpret_cast<const uint4*>(src) + q);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = in && c + e < l.width ? src[e] : (T)0.0f;
+  }
+  E out[PIECES][8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
     if (PIECES == 1) {
-      dst[i] = (E)v;
+      out[0][e] = (E)v[e];
     } else {
-      float left = as_float(v);
+      float left = as_float(v[e]);
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
-        const E e = (E)left;
-        dst[p * plane + i] = e;
-        left -= as_float(e);
+        out[p][e] = (E)left;
+        left -= as_float(out[p][e]);
       }
     }
   }
+#pragma unroll
+  for (int p = 0; p < PIECES; ++p) *reinterpret_cast<uint4*>((E*)l.dst + p * l.plane + i * 8) = *reinterpret_cast<const uint4*>(out[p]);
 }
-
-// x with its ignored rows zeroed, where one of them is not finite
-template <typename E>
-__global__ void __launch_bounds__(256) clean_kernel(const E* __restrict__ src, E* __restrict__ dst, int rows, int width,
-                                                    const long long* __restrict__ target, long long ignore,
-                                                    const float* __restrict__ strange) {
-  if (*strange == 0.0f) return;
-  const int pieces = width / 8;
-  const long long total = (long long)rows * pieces;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const bool in = target[i / pieces] != ignore;
-    reinterpret_cast<uint4*>(dst)[i] = in ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
+template <typename T, typename E, int PIECES>
+__global__ void __launch_bounds__(256) lay_out_kernel(const LayOut x, const LayOut w, long long ignore) {
+  before_all();
+  let_next();
+  const long long n = x.groups + w.groups;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    if (i < x.groups) lay_out_group<T, E, PIECES>(x, i, ignore);
+    else lay_out_group<T, E, PIECES>(w, i - x.groups, ignore);
   }
 }
 
-// ---- sums over splits and rows, in fixed order
+// the largest |up| of the rows that count, one block
+__global__ void __launch_bounds__(1024) largest_kernel(const float* __restrict__ up, const long long* __restrict__ y, long long ignore,
+                                                       int rows, float* largest) {
+  __shared__ float s[32];
+  before_all();
+  float v = 0;
+  for (int r = threadIdx.x; r < rows; r += 1024)
+    if (y[r] != ignore) v = fmaxf(v, fabsf(up[r]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  v = s[threadIdx.x];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if (threadIdx.x == 0) *largest = v;
+}
+
+// ---- sums over splits, in fixed order
 
 struct Join {
   const float* parts;  // [splits][count]
@@ -660,31 +800,13 @@ __device__ __forceinline__ void join_one(const Join& j, long long i) {
 }
 template <typename O>
 __global__ void __launch_bounds__(256) join_kernel(const Join a, const Join b) {
+  before_all();
+  let_next();
   const long long n = a.count + b.count;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
     if (i < a.count) join_one<O>(a, i);
     else join_one<O>(b, i - a.count);
   }
-}
-
-// db from the sums over 32 rows each: 32 classes a block
-template <typename O>
-__global__ void __launch_bounds__(1024) column_join_kernel(const float* __restrict__ sums, int slabs, int classes, float* acc, O* out,
-                                                           const float* back, int first) {
-  __shared__ float s[32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-  float v = 0;
-  if (c < classes)
-    for (int r = warp; r < slabs; r += 32) v += sums[(long long)r * classes + c];
-  s[warp][lane] = v;
-  __syncthreads();
-  if (warp || c >= classes) return;
-  v = 0;
-  for (int i = 0; i < 32; ++i) v += s[i][lane];
-  if (back) v *= *back;
-  if (!first) v += acc[c];
-  if (out) out[c] = (O)v;
-  else acc[c] = v;
 }
 
 // ------------------------------------------------------------------ plans
@@ -694,9 +816,9 @@ struct Config {
 };
 // Two SMs a tile where their tiles keep half of the pairs busy; below that tiles of one SM, narrow ones when even the wide
 // leave half of the SMs without one.
-Config pick(long long rows, long long cols) {
-  const int sms = device_sm_count();
-  if ((long long)div_up(rows, 256) * div_up(cols, 256) * 4 >= sms) return {2, 256};
+Config pick(long long rows, long long cols, int pieces) {
+  const int sms = device_sm_count(), wide = pieces == 1 ? 256 : 128;  // two accumulators of fp32 pieces: half the columns
+  if ((long long)div_up(rows, 256) * div_up(cols, wide) * 4 >= sms) return {2, wide};
   if ((long long)div_up(rows, 128) * div_up(cols, 128) * 2 >= sms) return {1, 128};
   return {1, 64};
 }
@@ -709,19 +831,12 @@ int launch_one(const Args& a, int items, cudaStream_t s) {
   const int rc = enable_smem(kernel, smem_bytes<CG, BN>());
   if (rc != DK_OK) return rc;
   const int clusters = device_sm_count() / CG;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((items < clusters ? items : clusters) * CG), cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem_bytes<CG, BN>(), cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr, cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, a);
-  return check_launch();
+  // the gradients' schedule is one of all clusters
+  return launch_after(kernel, (ROLE == kGrad || items > clusters ? clusters : items) * CG, kThreads, smem_bytes<CG, BN>(), CG, s, a);
 }
 template <int ROLE, typename E, int PIECES>
 int launch(const Config& c, const Args& a, int items, cudaStream_t s) {
-  if (c.cg == 2) return launch_one<2, 256, ROLE, E, PIECES>(a, items, s);
+  if (c.cg == 2) return launch_one<2, PIECES == 1 ? 256 : 128, ROLE, E, PIECES>(a, items, s);
   if (c.bn == 128) return launch_one<1, 128, ROLE, E, PIECES>(a, items, s);
   return launch_one<1, 64, ROLE, E, PIECES>(a, items, s);
 }
@@ -734,14 +849,17 @@ int pitch_of(int n) { return (n + 7) & ~7; }
 struct ForwardPlan {
   Config c;
   int tiles_m, tiles_n, slots;
+  bool few;
   size_t x, w, top, sum, all, picked, partial, bytes;
 };
 ForwardPlan forward_plan(int T, int D, int V, int dtype) {
   ForwardPlan p;
   Layout l;
-  p.c = pick(T, V);
+  p.c = pick(T, V, pieces_of(dtype));
   p.tiles_m = div_up(T, 128 * p.c.cg), p.tiles_n = div_up(V, p.c.bn), p.slots = p.tiles_n * groups_of(p.c);
-  const bool lay = laid_out(D, dtype);
+  p.few = few_rows(T, dtype);
+  if (p.few) p.slots = few_slots(V);
+  const bool lay = !p.few && laid_out(D, dtype);
   const size_t row = (size_t)pitch_of(D) * 2 * pieces_of(dtype);
   p.x = lay ? l.take(T * row) : 0, p.w = lay ? l.take(V * row) : 0;
   const size_t each = (size_t)p.slots * T * sizeof(float);
@@ -751,29 +869,50 @@ ForwardPlan forward_plan(int T, int D, int V, int dtype) {
   return p;
 }
 
-// dz of one piece; the whole call is one piece where it fits
-constexpr long long kPieceBytes = 128ll << 20;
+// dz of one piece; the whole call is one piece where it fits.  Fewer, larger pieces fill their last rounds of tiles better than smaller ones gain
+// from L2: 4096 rows, 21841 classes (179 MB) 758 us as one piece, 813 as two; 8192 rows, 65536 classes 6.68 ms with 256 MB,
+// 6.77 with 128, 7.10 with 64, 6.65 with 512.
+constexpr long long kPieceBytes = 256ll << 20;
 
 struct BackwardPlan {
   Config dz, grad;
   int tc, vc;                    // rows and classes of a piece: one of them is all there are
   int splits_w, per_w, splits_x, per_x;
-  size_t x, w, g, back, buffer, acc, acc_b, sums, parts_w, parts_x, bytes;
+  size_t x, w, largest, buffer, acc, acc_b, sums, parts_w, parts_x, bytes;
 };
 
 // splits of the two products so that a launch fills the SMs once where their tiles alone do not
-void split_products(BackwardPlan& p, int D) {
+void split_products(BackwardPlan& p, int D, int pieces) {
   const int clusters = clusters_of(p.grad), bm = 128 * p.grad.cg, tn = div_up(D, p.grad.bn);
   const long long tiles_w = (long long)div_up(p.vc, bm) * tn, tiles_x = (long long)div_up(p.tc, bm) * tn;
   const int blocks_w = div_up(p.tc, kBox), blocks_x = div_up(p.vc, kBox);
   const long long total = tiles_w * blocks_w + tiles_x * blocks_x;
-  // at least eight steps a split: less does not pay for writing and joining its sums
+  // at least 32 steps a split (of fp32, six products each, 8): the launch that joins the sums takes as long as some 20 steps
+  const int least = pieces == 1 ? 32 : 8;
   long long per = total / clusters + 1;
-  if (per < 8) per = 8;
+  if (per < least) per = least;
   p.per_w = (int)(per < blocks_w ? per : blocks_w), p.per_x = (int)(per < blocks_x ? per : blocks_x);
   p.splits_w = div_up(blocks_w, p.per_w), p.splits_x = div_up(blocks_x, p.per_x);
   p.per_w = div_up(blocks_w, p.splits_w), p.per_x = div_up(blocks_x, p.splits_x);
   p.splits_w = div_up(blocks_w, p.per_w), p.splits_x = div_up(blocks_x, p.per_x);
+}
+
+// the rounds of the two products' items that let all clusters end at about the same time
+Schedule schedule_of(const Product& dw, const Product& dx, int clusters) {
+  const int n_w = dw.tiles_m * dw.tiles_n * dw.splits, n_x = dx.tiles_m * dx.tiles_n * dx.splits;
+  Schedule c = {};
+  c.long_product = n_w == 0 || (n_x != 0 && dx.per > dw.per);
+  c.n_long = c.long_product ? n_x : n_w, c.n_short = c.long_product ? n_w : n_x;
+  const long long per_long = c.long_product ? dx.per : dw.per, per_short = c.long_product ? dw.per : dx.per;
+  const int rest = c.n_long % clusters;
+  long long dealt = 0;
+  while (dealt < c.n_short) {
+    // the clusters with one long item less go on until they would pass the others
+    if (rest == 0 || (c.short_more - c.short_less + 1) * per_short <= per_long) c.short_more += 1, dealt += clusters - rest;
+    else c.short_less += 1, dealt += rest;
+    if (rest == 0) c.short_less = c.short_more;
+  }
+  return c;
 }
 
 BackwardPlan backward_plan(int T, int D, int V, int dtype) {
@@ -792,20 +931,20 @@ BackwardPlan backward_plan(int T, int D, int V, int dtype) {
     const long long even = (long long)div_up(div_up(all, n), 256) * 256;
     side = even < all ? (int)even : all;
   }
-  p.dz = pick(p.tc, p.vc);
+  p.dz = pick(p.tc, p.vc, pieces);
   {
     // the two products have tc x D and vc x D tiles
-    const int sms = device_sm_count();
-    const long long pairs = (long long)(div_up(p.tc, 256) + div_up(p.vc, 256)) * div_up(D, 256);
+    const int sms = device_sm_count(), wide_n = pieces == 1 ? 256 : 128;
+    const long long pairs = (long long)(div_up(p.tc, 256) + div_up(p.vc, 256)) * div_up(D, wide_n);
     const long long wide = (long long)(div_up(p.tc, 128) + div_up(p.vc, 128)) * div_up(D, 128);
-    p.grad = pairs * 4 >= sms ? Config{2, 256} : wide * 2 >= sms ? Config{1, 128} : Config{1, 64};
+    p.grad = pairs * 4 >= sms ? Config{2, wide_n} : wide * 2 >= sms ? Config{1, 128} : Config{1, 64};
   }
-  split_products(p, D);
+  split_products(p, D, pieces);
   const bool lay = laid_out(D, dtype);
   const size_t row = (size_t)pitch_of(D) * 2 * pieces;
   p.x = l.take(T * row);  // laid out, or the copy without ignored rows
   p.w = lay ? l.take(V * row) : 0;
-  p.g = l.take((size_t)T * sizeof(float)), p.back = l.take(2 * sizeof(float));
+  p.largest = l.take(sizeof(float));
   p.buffer = l.take((size_t)p.tc * pitch_of(p.vc) * each);
   const bool cut_v = p.vc < V, cut_t = p.tc < T;
   p.acc = (cut_v || cut_t) && dtype != DK_F32 ? l.take((size_t)(cut_v ? T : V) * D * sizeof(float)) : 0;
@@ -834,13 +973,11 @@ int row_group(const Config& c, int D, int pieces) {
 template <typename T, typename E, int PIECES>
 int operands(const void*& x, const void*& w, char* to_x, char* to_w, const long long* y, const Shape& h, int dtype, cudaStream_t s) {
   if (!laid_out(h.D, dtype)) return DK_OK;
-  const int pitch = pitch_of(h.D);
-  lay_out_kernel<T, E, PIECES><<<blocks_for((long long)h.T * pitch), 256, 0, s>>>((const T*)x, (E*)to_x, h.T, h.D, pitch, y, h.ignore);
-  int rc = check_launch();
-  if (rc != DK_OK) return rc;
-  lay_out_kernel<T, E, PIECES><<<blocks_for((long long)h.V * pitch), 256, 0, s>>>((const T*)w, (E*)to_w, h.V, h.D, pitch, nullptr, 0);
+  const int per_row = pitch_of(h.D) / 8;
+  LayOut lx = {x, to_x, (long long)h.T * per_row, h.D, per_row, (long long)h.T * per_row * 8, y};
+  LayOut lw = {w, to_w, (long long)h.V * per_row, h.D, per_row, (long long)h.V * per_row * 8, nullptr};
   x = to_x, w = to_w;
-  return check_launch();
+  return launch_after(lay_out_kernel<T, E, PIECES>, blocks_for(lx.groups + lw.groups), 256, 0, 1, s, lx, lw, h.ignore);
 }
 template <typename E, int PIECES>
 bool operand_map(CUtensorMap* tm, const void* p, int rows, int width, int pitch, int box_rows = kBox) {
@@ -854,6 +991,12 @@ int forward(const void* x, const void* w, const void* b, const long long* y, voi
   const ForwardPlan p = forward_plan(h.T, h.D, h.V, dtype);
   if (!ws || ws_bytes < p.bytes) return DK_ERR_WORKSPACE;
   char* m = (char*)ws;
+  if (p.few) {
+    const Partials<float> part = {(float*)(m + p.top), (float*)(m + p.sum), (float*)(m + p.all), (float*)(m + p.picked)};
+    double* partial = (double*)(m + p.partial);
+    const int rc = launch_few_rows<T>(x, w, b, y, part, combine_count(partial, h.T), h, s);
+    return rc != DK_OK ? rc : launch_combine<float>(part, y, p.slots, loss, saved, partial, h, s);
+  }
   int rc = operands<T, E, PIECES>(x, w, m + p.x, m + p.w, y, h, dtype, s);
   if (rc != DK_OK) return rc;
   Args a = {};
@@ -863,7 +1006,7 @@ int forward(const void* x, const void* w, const void* b, const long long* y, voi
   a.tiles_m = p.tiles_m, a.tiles_n = p.tiles_n, a.group = row_group(p.c, h.D, PIECES);
   a.bias = b, a.target = y, a.ignore = h.ignore;
   a.top = (float*)(m + p.top), a.sum = (float*)(m + p.sum), a.all = h.smoothing != 0.0 ? (float*)(m + p.all) : nullptr;
-  a.picked = (float*)(m + p.picked);
+  a.picked = (float*)(m + p.picked), a.done = combine_count((double*)(m + p.partial), h.T);
   if ((long long)p.tiles_m * p.tiles_n > 0x3fffffff) return DK_ERR_UNSUPPORTED;
   rc = launch<kStats, E, PIECES>(p.c, a, p.tiles_m * p.tiles_n, s);
   if (rc != DK_OK) return rc;
@@ -877,24 +1020,27 @@ int backward(const void* up, const void* x, const void* w, const void* b, const 
   const BackwardPlan p = backward_plan(h.T, h.D, h.V, dtype);
   if (!ws || ws_bytes < p.bytes) return DK_ERR_WORKSPACE;
   char* m = (char*)ws;
-  float *g = (float*)(m + p.g), *back = dtype == DK_F16 ? (float*)(m + p.back) : nullptr;
   const float* stat = (const float*)saved;
-  int rc = launch_rows<float>(up, y, saved, g, back, h, s);
+  float* largest = dtype == DK_F16 && h.reduction == DK_REDUCE_NONE ? (float*)(m + p.largest) : nullptr;
+  int rc = DK_OK;
+  if (largest) rc = launch_after(largest_kernel, 1, 1024, 0, 1, s, (const float*)up, y, h.ignore, h.T, largest);
   if (rc != DK_OK) return rc;
   Args a = {};
   const int pitch = pitch_of(h.D);
   if (laid_out(h.D, dtype)) {
     rc = operands<T, E, PIECES>(x, w, m + p.x, m + p.w, y, h, dtype, s);
+    if (rc != DK_OK) return rc;
   } else if (dw) {
-    a.strange = stat + h.T + 1;
-    clean_kernel<E><<<blocks_for((long long)h.T * h.D / 8), 256, 0, s>>>((const E*)x, (E*)(m + p.x), h.T, h.D, y, h.ignore, a.strange);
-    rc = check_launch();
+    a.strange = stat + 2ll * h.T + 1;
   }
-  if (rc != DK_OK) return rc;
   if (!operand_map<E, PIECES>(&a.x, x, h.T, h.D, pitch) || !operand_map<E, PIECES>(&a.w, w, h.V, h.D, pitch) ||
       !operand_map<E, PIECES>(&a.x_clean, m + p.x, h.T, h.D, pitch))
     return DK_ERR_CUDA;
-  a.depth = div_up(h.D, kBox), a.bias = b, a.ignore = h.ignore, a.back = back;
+  a.depth = div_up(h.D, kBox), a.bias = b, a.ignore = h.ignore, a.all_classes = h.V;
+  a.up = {(const float*)up, stat + 2ll * h.T, largest, h.reduction, 1.0f};
+  // up to one half: beyond, p unit would leave fp16's range
+  if (h.reduction != DK_REDUCE_NONE)
+    a.up.unit = (float)((dtype == DK_F16 ? 16384.0 : 1.0) / (h.smoothing <= 0.5 ? 1.0 - h.smoothing : 1.0));
   a.smooth_each = (float)(h.smoothing / h.V), a.smooth_own = (float)(1.0 - h.smoothing);
   a.column_sums = db ? (float*)(m + p.sums) : nullptr;
   const bool cut_v = p.vc < h.V;
@@ -909,7 +1055,10 @@ int backward(const void* up, const void* x, const void* w, const void* b, const 
         return DK_ERR_CUDA;
       a.rows = rows, a.classes = classes, a.row0 = t0, a.class0 = v0;
       a.tiles_m = div_up(rows, 128 * p.dz.cg), a.tiles_n = div_up(classes, p.dz.bn), a.group = row_group(p.dz, h.D, PIECES);
-      a.target = y + t0, a.lse2 = stat + t0, a.g = g + t0;
+      a.target = y + t0, a.ref = stat + t0, a.inv = stat + h.T + t0;
+      if (h.reduction == DK_REDUCE_NONE) a.up.up = (const float*)up + t0;
+      if (a.strange && first_t && first_v) a.dirty = x, a.clean = m + p.x, a.width = h.D, a.up_rows = h.T, a.target_all = y;
+      else a.clean = nullptr;
       rc = launch<kDz, E, PIECES>(p.dz, a, a.tiles_m * a.tiles_n, s);
       if (rc != DK_OK) return rc;
       // dw [classes][D] sums over rows, dx [rows][D] over classes; the running sums of fp32 gradients are the gradients
@@ -939,25 +1088,13 @@ int backward(const void* up, const void* x, const void* w, const void* b, const 
           px.acc = (float*)(m + p.parts_x), px.out = nullptr, px.first = 1;
         }
       }
-      a.dw = pw, a.dx = px;
-      if (dw || dx) {
-        const long long items = (long long)pw.tiles_m * tn * pw.splits + (long long)px.tiles_m * tn * px.splits;
-        if (items > 0x3fffffff) return DK_ERR_UNSUPPORTED;
-        rc = launch<kGrad, E, PIECES>(p.grad, a, (int)items, s);
-        if (rc != DK_OK) return rc;
-      }
-      if (jw.count + jx.count > 0) {
-        join_kernel<T><<<blocks_for(jw.count + jx.count), 256, 0, s>>>(jw, jx);
-        rc = check_launch();
-        if (rc != DK_OK) return rc;
-      }
-      if (db) {
-        float* acc = cut_v ? nullptr : (float*)(m + p.acc_b);
-        column_join_kernel<T><<<div_up(classes, 32), 1024, 0, s>>>(a.column_sums, div_up(rows, 32), classes, acc,
-                                                                   last_t ? (T*)db + v0 : nullptr, back, first_t);
-        rc = check_launch();
-        if (rc != DK_OK) return rc;
-      }
+      a.dw = pw, a.dx = px, a.schedule = schedule_of(pw, px, clusters_of(p.grad));
+      if (db) a.acc_b = cut_v ? nullptr : (float*)(m + p.acc_b), a.out_b = last_t ? (T*)db + v0 : nullptr, a.first_b = first_t;
+      const long long items = (long long)pw.tiles_m * tn * pw.splits + (long long)px.tiles_m * tn * px.splits;
+      if (items > 0x3fffffff) return DK_ERR_UNSUPPORTED;
+      rc = launch<kGrad, E, PIECES>(p.grad, a, (int)items, s);
+      if (rc == DK_OK && jw.count + jx.count > 0) rc = launch_after(join_kernel<T>, blocks_for(jw.count + jx.count), 256, 0, 1, s, jw, jx);
+      if (rc != DK_OK) return rc;
     }
   return DK_OK;
 }

@@ -671,7 +671,7 @@ inline Tensor aligned(const Tensor& t) {
 
 struct LinearCrossEntropyBackward : public Node {
   SavedVariable input, weight, bias, target;
-  Tensor saved;  // log-sum-exp of the rows and their count; not visible outside
+  Tensor saved;  // what the rows' probabilities are made of, and their count; not visible outside
   bool has_bias = false;
   CrossEntropyArgs a;
   std::vector<int64_t> in_sizes, out_sizes;
@@ -733,7 +733,7 @@ Tensor linear_cross_entropy(const Tensor& input, const Tensor& weight, const Ten
     if (bias.defined()) b = bias.contiguous();
     const at::ScalarType type = code == DK_F64 ? at::kDouble : at::kFloat;
     out = empty_of(x, a.reduction == DK_REDUCE_NONE ? target.sizes() : at::IntArrayRef(), type);
-    if (grad) saved = empty_of(x, {(int64_t)rows + 2}, type);
+    if (grad) saved = empty_of(x, {2 * (int64_t)rows + 2}, type);
     if (rows > 0) {
       const size_t bytes = lib.dk_linear_cross_entropy_forward_workspace_bytes(rows, features, classes, code);
       Tensor ws = workspace(bytes, x);

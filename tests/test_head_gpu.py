@@ -148,7 +148,7 @@ def check(x, w, y, b, up, where="", device="cpu", **kw):
     return got
 
 
-SIZES = [(1, 8, 2), (1, 1280, 1000), (2, 1, 1), (31, 24, 7), (33, 33, 65), (127, 64, 130), (128, 128, 256), (129, 200, 257), (300, 96, 1000),
+SIZES = [(1, 8, 2), (2, 100, 5000), (3, 256, 1200), (4, 72, 4800), (5, 64, 5001), (8, 33, 700), (1, 1280, 1000), (2, 1, 1), (31, 24, 7), (33, 33, 65), (127, 64, 130), (128, 128, 256), (129, 200, 257), (300, 96, 1000),
          (257, 65, 1031), (64, 520, 4099), (1030, 40, 64)]
 
 
@@ -247,6 +247,24 @@ def test_large_and_small_logits():
         x, w, y, b, up = make(50, 64, 200, dtype, seed=3)
         check(x * 16, w * 4, y, b, up)
         check(x * 0, w, y, b, up)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_losses_near_zero(rows, dtype):
+    """The row's own logit far above the others: the loss is log(1 + e), not the difference of two large numbers.  Logits are
+    whole numbers (exact), e is off by 2^-22 of itself, 1 + e by 2^-24, its logarithm by 2^-23 of itself and twice that
+    in steps; 60 losses of a sum change nothing, the mean is one of equal values."""
+    for gap in (3.0, 8.0, 11.0):
+        x = torch.zeros(rows, 16)
+        x[:, 0] = 1.0
+        w = torch.zeros(2, 16)
+        w[0, 0], w[1, 0] = 20.0, 20.0 - gap
+        y = torch.zeros(rows, dtype=torch.int64)
+        dt = H.DTYPES[dtype]
+        got = functions().linear_cross_entropy(x.to(dt).to(DEV), w.to(dt).to(DEV), y.to(DEV)).item()
+        want = torch.log1p(torch.exp(torch.tensor(-gap, dtype=torch.double))).item()
+        assert abs(got - want) < 2.0 ** -23 + 2.0 ** -21 * want
 
 
 def test_leading_dimensions_views_and_dtypes():
@@ -403,3 +421,35 @@ def test_head_and_dropout_together_as_a_training_step():
         assert loss.dtype == torch.float32
         loss.backward()
     assert head.weight.grad.dtype == torch.float32
+
+
+def test_calls_from_threads_that_have_not_used_the_gpu_yet():
+    """Forward, and backward on autograd's thread, as the first thing a process and its threads do; two threads at once."""
+    import subprocess
+    import sys
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import sys, threading
+sys.path[:0] = [%r, %r]
+import torch
+import head_oracle as H
+import test_head_gpu as T
+cases = [T.make(60, 32, 50, "bf16", seed=s) for s in range(4)]
+wrong = []
+def work(case):
+    try:
+        for _ in range(20):
+            T.check(*case)
+    except BaseException as e:
+        wrong.append(e)
+x, w, y, b, up = (t.cuda() for t in cases[0])
+x.requires_grad_(True)
+torch.autograd.grad(T.functions().linear_cross_entropy(x, w, y, b), x, up)
+threads = [threading.Thread(target=work, args=(c,)) for c in cases]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert not wrong, wrong
+""" % (os.path.join(root, "deformable-kernels_b200"), os.path.join(root, "tests"))
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
+    assert out.returncode == 0, out.stderr[-2000:]
