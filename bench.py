@@ -265,12 +265,32 @@ def build_mobilenet_dk():
     return model, replaced
 
 
+class ClassifierStep(torch.nn.Module):
+    """A torchvision classifier and its loss: dropout, last linear layer and softmax cross entropy as this package's
+    LinearCrossEntropy, which stores neither a mask nor logits.  Takes over the classifier's parameters."""
+
+    def __init__(self, model):
+        super().__init__()
+        from deformable_kernels.modules import LinearCrossEntropy
+        drop, linear = model.classifier
+        self.head = LinearCrossEntropy(linear.in_features, linear.out_features, bias=linear.bias is not None, dropout=drop.p)
+        self.head.load_state_dict(linear.state_dict())
+        model.classifier = torch.nn.Identity()
+        self.net = model
+
+    def forward(self, x, labels):
+        return self.head(self.net(x), labels)
+
+
 def run_training_step(args, rank, world, local, dev):
     """forward + backward + SGD step of MobileNetV2-DK on synthetic 224x224 images, fp16
     autocast, global batch sharded over the ranks, gradients all-reduced by NCCL through DDP."""
     import torch.distributed as dist
     torch.manual_seed(0)
     model, replaced = build_mobilenet_dk()
+    fused = args.head == "fused"
+    if fused:
+        model = ClassifierStep(model)
     model = model.to(dev).to(memory_format=torch.contiguous_format)
     if world > 1:
         model = torch.nn.parallel.DistributedDataParallel(model, device_ids=[local])
@@ -286,12 +306,12 @@ def run_training_step(args, rank, world, local, dev):
         # forward and backward of the whole network as two CUDA graphs (the operators capture: they enqueue on the
         # current stream, never synchronise and take their scratch from the caller); loss, scaler and optimizer stay eager
         with torch.autocast("cuda", dtype=torch.float16, cache_enabled=False):
-            model = torch.cuda.make_graphed_callables(model, (x.clone(),))
+            model = torch.cuda.make_graphed_callables(model, (x.clone(), labels.clone()) if fused else (x.clone(),))
 
     def step():
         opt.zero_grad(set_to_none=not graphed)
         with torch.autocast("cuda", dtype=torch.float16, cache_enabled=not graphed):
-            loss = loss_fn(model(x), labels)
+            loss = model(x, labels) if fused else loss_fn(model(x), labels)
         scaler.scale(loss).backward()
         scaler.step(opt)
         scaler.update()
@@ -368,7 +388,7 @@ def run_training_step(args, rank, world, local, dev):
             "vs_baseline": None, "dtype": "f16 autocast, f32 master weights", "data": "synthetic",
             "config": {"workload": "cfg5: MobileNetV2-1.0 with %d DeformKernel2d layers (scope 4x4), 224x224, SGD step, "
                                    "DDP/NCCL gradient all-reduce" % replaced, "per_gpu_batch": per_gpu,
-                       "cuda_graph": graphed},
+                       "head": args.head, "cuda_graph": graphed},
             "loss": float(loss.item()), "clocks": clocks, "peak_mem_GB": round(torch.cuda.max_memory_allocated() / 1e9, 1)}))
 
 
@@ -517,6 +537,8 @@ def main():
                     help="sweep: the DK layer sweep (headline); train: MobileNetV2-DK training step, global batch 1024; "
                          "dcn: one DK + DCN layer (BASELINE config 4)")
     ap.add_argument("--global-batch", type=int, default=1024)
+    ap.add_argument("--head", default="fused", choices=["fused", "torch"],
+                    help="classifier and loss of the training step: LinearCrossEntropy, or stock modules")
     ap.add_argument("--cuda-graph", action="store_true",
                     help="train workload, one GPU: run the network's forward and backward as captured CUDA graphs (the sweep replays "
                          "its step as a CUDA graph by default, see --eager)")

@@ -329,7 +329,8 @@ __global__ void __launch_bounds__(1024) combine_kernel(Partials<A> p, const long
   const int r = blockIdx.x * 32 + lane;
   before_all();
   A top = minus_inf<A>(), sum = (A)0, all = (A)0;
-  if (r < h.T)
+  if (r < h.T) {
+#pragma unroll 4
     for (int s = warp; s < slots; s += warps) {
       const long long at = (long long)s * h.T + r;
       const A t = p.top[at], n = fmax(top, t), ref = n == minus_inf<A>() ? (A)0 : n;
@@ -337,6 +338,7 @@ __global__ void __launch_bounds__(1024) combine_kernel(Partials<A> p, const long
       top = n;
       if (h.smoothing != 0.0) all += p.all[at];
     }
+  }
   s_top[lane][warp] = top, s_sum[lane][warp] = sum, s_all[lane][warp] = all;
   __syncthreads();
   if (warp) return;

@@ -10,7 +10,8 @@
 //
 // fp32 operands are three bf16 pieces each (8 bits a piece, 24 in all).  A stage holds one piece of both; the six products of
 // pieces that reach 2^-24 are taken from three stages, that of the leading pieces into one accumulator, the five
-// small ones into another: the additions of the tensor cores cut, and a cut of the small sum costs nothing.
+// small ones into another: the additions of the tensor cores cut, and a cut of the small sum costs nothing.  After every eight steps
+// the epilogue adds both to sums in registers, which round, so that no more than 32 cuts meet in one value.
 #include <math_constants.h>
 
 #include <type_traits>
@@ -139,6 +140,22 @@ __device__ __forceinline__ void wait_ld(float (&r)[32]) {
                  "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15]), "+r"(u[16]), "+r"(u[17]), "+r"(u[18]),
                  "+r"(u[19]), "+r"(u[20]), "+r"(u[21]), "+r"(u[22]), "+r"(u[23]), "+r"(u[24]), "+r"(u[25]), "+r"(u[26]), "+r"(u[27]),
                  "+r"(u[28]), "+r"(u[29]), "+r"(u[30]), "+r"(u[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void ld16(float (&r)[16], unsigned a) {
+  unsigned* u = reinterpret_cast<unsigned*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+        "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(a));
+}
+__device__ __forceinline__ void wait_ld(float (&r)[16]) {
+  unsigned* u = reinterpret_cast<unsigned*>(r);
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]), "+r"(u[8]), "+r"(u[9]),
+                 "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15])
                :
                : "memory");
 }
@@ -349,20 +366,16 @@ __device__ __forceinline__ void product(unsigned d, uint64_t a, uint64_t b, unsi
   for (int q = 0; q < 4; ++q) mma_ss<CG>(d + at, a + (uint64_t)(q * step_a >> 4), b + (uint64_t)(q * step_b >> 4), idesc, !fresh || q > 0);
 }
 
-// 32 columns of the finished accumulator
-template <int BN, int PIECES>
-__device__ __forceinline__ void take(float (&v)[32], unsigned a) {
-  ld32(v, a);
-  if (PIECES == 1) {
-    wait_ld(v);
-  } else {
-    float small[32];
-    ld32(small, a + BN);
-    wait_ld(v);
-    wait_ld(small);
+// 16 columns of both sums of an fp32 accumulator, added to v (set: stored)
+template <int BN>
+__device__ __forceinline__ void take_both(float* v, unsigned a, bool set) {
+  float lead[16], small[16];
+  ld16(lead, a);
+  ld16(small, a + BN);
+  wait_ld(lead);
+  wait_ld(small);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] += small[j];
-  }
+  for (int j = 0; j < 16; ++j) v[j] = set ? lead[j] + small[j] : v[j] + (lead[j] + small[j]);
 }
 
 // ---- the kernel
@@ -375,6 +388,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
   constexpr int kGroups = BN >= 128 ? 2 : 1;       // epilogue warps side by side
   constexpr int kWide = BN / kGroups;              // columns of an epilogue warp
   constexpr int kAcc = PIECES == 1 ? BN : 2 * BN;  // columns of an accumulator
+  constexpr int kChunk = PIECES == 1 ? 1 << 30 : 8;  // steps between two takings of the accumulator
+  static_assert(PIECES == 1 || kWide == 64, "the sums of a row are 64 registers");
   static_assert(2 * kAcc <= 512, "two accumulators in TMEM");
   SharedTail& t = *reinterpret_cast<SharedTail*>(smem + kStages * kStage + 8 * kStageWarp);
   const unsigned base = smem_u32(smem);
@@ -446,46 +461,49 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
     if (rank == 0) {
       const bool one = tc::elect_one();
       constexpr unsigned kDesc = (1u << 4) | type_bits<E>() | ((unsigned)(BN >> 3) << 17) | ((unsigned)(128 * CG >> 4) << 24);
-      int fill = 0, tile = 0;
+      int fill = 0, round = 0;
       Item it;
-      for (; item_of<ROLE>(a, cluster, clusters, tile, it); ++tile) {
+      for (int tile = 0; item_of<ROLE>(a, cluster, clusters, tile, it); ++tile) {
         // both operands of the logits are K-major; W and x of the gradients are MN-major, dz is either
         const bool ta = ROLE == kGrad && it.product == 0, tb = ROLE == kGrad;
         const unsigned idesc = kDesc | ((unsigned)ta << 15) | ((unsigned)tb << 16);
         const unsigned lead = kBoxBytes, step_a = ta ? 2048 : 32, step_b = tb ? 2048 : 32;
-        const int b = tile & 1;
-        bool gone = wait(smem_u32(&t.acc_empty[b]), ((tile >> 1) & 1) ^ 1, abort_flag);
-        tc::fence_after();
-        const unsigned d = tmem + b * kAcc;
-        for (int k = 0; k < it.count; ++k, fill += PIECES) {
-          uint64_t da[PIECES], db[PIECES];
+        for (int k0 = 0; k0 < it.count; k0 += kChunk, ++round) {
+          const int b = round & 1, end = it.count - k0 < kChunk ? it.count : k0 + kChunk;
+          bool gone = wait(smem_u32(&t.acc_empty[b]), ((round >> 1) & 1) ^ 1, abort_flag);
+          tc::fence_after();
+          const unsigned d = tmem + b * kAcc;
+          for (int k = k0; k < end; ++k, fill += PIECES) {
+            uint64_t da[PIECES], db[PIECES];
 #pragma unroll
-          for (int p = 0; p < PIECES; ++p) {
-            const int s = (fill + p) % kStages;
-            gone = wait(smem_u32(&t.full[s]), ((fill + p) / kStages) & 1, abort_flag);
-            if (gone) break;
-            tc::fence_after();
-            const unsigned sa = base + s * kStage;
-            da[p] = swizzled(sa, lead, 1024), db[p] = swizzled(sa + 128 * 128, lead, 1024);
-            if (one) {
-              // product (i, j) of pieces i + j <= 2 as soon as the later of the two has landed
+            for (int p = 0; p < PIECES; ++p) {
+              const int s = (fill + p) % kStages;
+              gone = wait(smem_u32(&t.full[s]), ((fill + p) / kStages) & 1, abort_flag);
+              if (gone) break;
+              tc::fence_after();
+              const unsigned sa = base + s * kStage;
+              da[p] = swizzled(sa, lead, 1024), db[p] = swizzled(sa + 128 * 128, lead, 1024);
+              if (one) {
+                // product (i, j) of pieces i + j <= 2 as soon as the later of the two has landed
 #pragma unroll
-              for (int i = 0; i <= p; ++i) {
-                if (PIECES == 1 || i + p <= 2) product<CG>(d, da[p], db[i], p == 0 ? 0 : BN, idesc, step_a, step_b, k == 0 && (p == 0 || (p == 1 && i == 0)));
-                if (i != p && i + p <= 2) product<CG>(d, da[i], db[p], BN, idesc, step_a, step_b, false);
+                for (int i = 0; i <= p; ++i) {
+                  if (PIECES == 1 || i + p <= 2) product<CG>(d, da[p], db[i], p == 0 ? 0 : BN, idesc, step_a, step_b,
+                                                            k == k0 && (p == 0 || (p == 1 && i == 0)));
+                  if (i != p && i + p <= 2) product<CG>(d, da[i], db[p], BN, idesc, step_a, step_b, false);
+                }
               }
+              __syncwarp();
+            }
+            if (gone) continue;
+            if (one) {
+#pragma unroll
+              for (int p = 0; p < PIECES; ++p) commit<CG>(smem_u32(&t.empty[(fill + p) % kStages]));
             }
             __syncwarp();
           }
-          if (gone) continue;
-          if (one) {
-#pragma unroll
-            for (int p = 0; p < PIECES; ++p) commit<CG>(smem_u32(&t.empty[(fill + p) % kStages]));
-          }
+          if (one && !gone) commit<CG>(smem_u32(&t.acc_full[b]));
           __syncwarp();
         }
-        if (one && !gone) commit<CG>(smem_u32(&t.acc_full[b]));
-        __syncwarp();
       }
     }
   } else if (warp == 3) {
@@ -501,13 +519,22 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
     const unsigned stage = base + kStages * kStage + (warp - 4) * kStageWarp;
     const unsigned lanes = (unsigned)(32 * sub) << 16;
     constexpr float kL2 = (float)kLog2e;
-    int tile = 0;
+    // the accumulator `b` is taken: the mma may write it again
+    auto release = [&](int b) {
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        const unsigned bar = smem_u32(&t.acc_empty[b]);
+        if (CG == 1) ring::mbar_arrive(bar);
+        else arrive_cluster(map_rank(bar, 0));
+      }
+    };
+    int round = 0;
     Item it;
-    for (; item_of<ROLE>(a, cluster, clusters, tile, it); ++tile) {
-      const int b = tile & 1;
+    for (int tile = 0; item_of<ROLE>(a, cluster, clusters, tile, it); ++tile) {
       const int row_base = (it.m * CG + (int)rank) * 128 + 32 * sub, row = row_base + lane;
       const int col_base = it.n * BN + grp * kWide;
-      float* bias = t.bias[b];
+      float* bias = t.bias[tile & 1];
       long long y = -1;
       float ref = 0, inv = 0, g = 0;
       bool live = false;
@@ -528,16 +555,43 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
       // the row's own class as a column of this warp, -1: elsewhere
       const long long far = y - a.class0 - col_base;
       const int own = far >= 0 && far < kWide ? (int)far : -1;
-      (void)wait(smem_u32(&t.acc_full[b]), (tile >> 1) & 1, abort_flag);
-      tc::fence_after();
+      const int b = round & 1;
       const unsigned d = tmem + lanes + b * kAcc + grp * kWide;
+      float got[PIECES == 1 ? 1 : 2][32];  // fp32: the sums
+      if (PIECES == 1) {
+        (void)wait(smem_u32(&t.acc_full[b]), (round >> 1) & 1, abort_flag);
+        tc::fence_after();
+        ++round;
+      } else {
+        for (int k = 0; k < it.count; k += kChunk, ++round) {
+          const int bk = round & 1;
+          (void)wait(smem_u32(&t.acc_full[bk]), (round >> 1) & 1, abort_flag);
+          tc::fence_after();
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            __syncwarp();
+            take_both<BN>(&got[PIECES == 1 ? 0 : h >> 1][(h & 1) * 16], tmem + lanes + bk * kAcc + grp * kWide + 16 * h, k == 0);
+          }
+          release(bk);
+        }
+      }
+      // 32 columns from c on
+      auto columns = [&](float (&v)[32], int c) {
+        if (PIECES == 1) {
+          __syncwarp();
+          ld32(v, d + c);
+          wait_ld(v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = c == 0 ? got[0][j] : got[PIECES == 1 ? 0 : 1][j];
+        }
+      };
       if (ROLE == kStats) {
         float top = -CUDART_INF_F, sum = 0, all = 0, picked = 0;
-#pragma unroll 1
+#pragma unroll(PIECES == 1 ? 1 : 2)
         for (int c0 = 0; c0 < kWide; c0 += 32) {
           float z[32];
-          __syncwarp();
-          take<BN, PIECES>(z, d + c0);
+          columns(z, c0);
           const float4* bp = reinterpret_cast<const float4*>(bias + grp * kWide + c0);
           float most = -CUDART_INF_F;
 #pragma unroll
@@ -576,9 +630,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           const bool inside = row_base < a.rows && col_base + c0 < a.classes;
           if (!inside) break;  // of the whole warp
           float v[2][32];
-          __syncwarp();
-          take<BN, PIECES>(v[0], d + c0);
-          take<BN, PIECES>(v[1], d + c0 + 32);
+          columns(v[0], c0);
+          columns(v[1], c0 + 32);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float4* bp = reinterpret_cast<const float4*>(bias + grp * kWide + c0 + 32 * h);
@@ -640,12 +693,11 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         const bool out16 = PIECES == 1 && p.out;  // 16-bit results; else fp32, to the gradient or to the sums
         float* to32 = p.out ? (float*)p.out : acc;
         const bool vec = (p.N & (out16 ? 7 : 3)) == 0;
-#pragma unroll 1
+#pragma unroll(PIECES == 1 ? 1 : 2)
         for (int c0 = 0; c0 < kWide; c0 += 32) {
           if (row_base >= p.M || col_base + c0 >= p.N) break;  // of the whole warp
           float v[32];
-          __syncwarp();
-          take<BN, PIECES>(v, d + c0);
+          columns(v, c0);
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             sts16(staged(stage, lane, q), __float_as_uint(v[4 * q] * back), __float_as_uint(v[4 * q + 1] * back),
@@ -682,13 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           }
         }
       }
-      tc::fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        const unsigned bar = smem_u32(&t.acc_empty[b]);
-        if (CG == 1) ring::mbar_arrive(bar);
-        else arrive_cluster(map_rank(bar, 0));
-      }
+      if (PIECES == 1) release(b);
     }
     if (ROLE == kDz && lane == 0) stores_done();
   }

@@ -453,3 +453,38 @@ assert not wrong, wrong
 """ % (os.path.join(root, "deformable-kernels_b200"), os.path.join(root, "tests"))
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
     assert out.returncode == 0, out.stderr[-2000:]
+
+
+def test_training_step_of_the_bench_with_the_fused_head():
+    """MobileNetV2-DK with its classifier and loss as LinearCrossEntropy against the same network with the stock modules:
+    fp32, running statistics (no dropout then), loss and the gradients at both ends of the network."""
+    import bench
+    old = (torch.backends.cudnn.allow_tf32, torch.backends.cuda.matmul.allow_tf32)
+    torch.backends.cudnn.allow_tf32 = torch.backends.cuda.matmul.allow_tf32 = False
+    try:
+        torch.manual_seed(0)
+        stock, _ = bench.build_mobilenet_dk()
+        stock = stock.to(DEV).eval()
+        with torch.no_grad():
+            stock.classifier[1].weight.normal_(0, 0.05)
+        x = torch.randn(4, 3, 96, 96, device=DEV)
+        y = torch.randint(0, 1000, (4,), device=DEV)
+        loss = torch.nn.functional.cross_entropy(stock(x), y)
+        loss.backward()
+        want = {n: p.grad.clone() for n, p in stock.named_parameters() if p.grad is not None}
+        stock.zero_grad(set_to_none=True)
+        fused = bench.ClassifierStep(stock).eval().to(DEV)
+        loss2 = fused(x, y)
+        loss2.backward()
+        assert abs(loss.item() - loss2.item()) < 1e-5 * abs(loss.item())
+        for mine, theirs in (("head.weight", "classifier.1.weight"), ("head.bias", "classifier.1.bias"),
+                             ("net.features.18.0.weight", "features.18.0.weight"),
+                             ("net.features.1.conv.0.0.inner_conv.weight", "features.1.conv.0.0.inner_conv.weight")):
+            a, b = fused.get_parameter(mine).grad.double(), want[theirs].double()
+            assert (a - b).norm() < 1e-4 * b.norm(), mine
+        fused.train()
+        with torch.autocast("cuda", dtype=torch.float16):
+            losses = [fused(x, y) for _ in range(2)]
+        assert all(v.dtype == torch.float32 and torch.isfinite(v) for v in losses)
+    finally:
+        torch.backends.cudnn.allow_tf32, torch.backends.cuda.matmul.allow_tf32 = old
