@@ -529,29 +529,52 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         else arrive_cluster(map_rank(bar, 0));
       }
     };
+    // What a tile needs from global memory is asked for a tile ahead: the row's class and statistics, and the thread's share of what is added to
+    // the logits (-inf outside, where the product is zero).
+    constexpr int kShare = (BN + 128 * kGroups - 1) / (128 * kGroups);
+    struct Ahead {
+      long long y;
+      float ref, inv, up, bias[kShare];
+    };
+    auto ask = [&](Ahead& n, const Item& it) {
+      if (ROLE == kGrad) return;
+#pragma unroll
+      for (int i = 0; i < kShare; ++i) {
+        const int v = it.n * BN + (int)threadIdx.x - 128 + i * 128 * kGroups;
+        n.bias[i] = v < a.classes ? (a.bias ? (PIECES == 1 ? (float)((const E*)a.bias)[a.class0 + v] : ((const float*)a.bias)[a.class0 + v]) : 0.0f)
+                                  : -CUDART_INF_F;
+      }
+      const int row = (it.m * CG + (int)rank) * 128 + 32 * sub + lane;
+      n.y = a.ignore;
+      if (row < a.rows) {
+        n.y = a.target[row];
+        if (ROLE == kDz) n.ref = a.ref[row], n.inv = a.inv[row], n.up = a.up.reduction == DK_REDUCE_NONE ? a.up.up[row] : 1.0f;
+      }
+    };
+    const float unit = ROLE == kDz ? upstream_unit(a.up) : 0.0f, back = ROLE == kGrad ? upstream_back(a.up) : 0.0f;
     int round = 0;
-    Item it;
-    for (int tile = 0; item_of<ROLE>(a, cluster, clusters, tile, it); ++tile) {
+    Item it, next;
+    Ahead now = {}, ahead = {};
+    bool more = item_of<ROLE>(a, cluster, clusters, 0, next);
+    if (more) ask(ahead, next);
+    for (int tile = 0; more; ++tile) {
+      it = next, now = ahead;
       const int row_base = (it.m * CG + (int)rank) * 128 + 32 * sub, row = row_base + lane;
       const int col_base = it.n * BN + grp * kWide;
       float* bias = t.bias[tile & 1];
-      long long y = -1;
-      float ref = 0, inv = 0, g = 0;
-      bool live = false;
       if (ROLE != kGrad) {
-        // what is added to the logits; -inf outside, where the product is zero
-        for (int c = threadIdx.x - 128; c < BN; c += 128 * kGroups) {
-          const int v = it.n * BN + c;
-          bias[c] = v < a.classes ? (a.bias ? (PIECES == 1 ? (float)((const E*)a.bias)[a.class0 + v] : ((const float*)a.bias)[a.class0 + v]) : 0.0f)
-                                  : -CUDART_INF_F;
-        }
-        if (row < a.rows) {
-          y = a.target[row];
-          if (ROLE == kDz) ref = a.ref[row], inv = a.inv[row], g = upstream_row(a.up, row, y, a.ignore, a.all_classes), live = y != a.ignore;
-        }
+        // the other half is read until the next tile's barrier
+#pragma unroll
+        for (int i = 0; i < kShare; ++i)
+          if ((int)threadIdx.x - 128 + i * 128 * kGroups < BN) bias[(int)threadIdx.x - 128 + i * 128 * kGroups] = now.bias[i];
         __syncwarp();
         asm volatile("bar.sync 1, %0;\n" ::"n"(128 * kGroups) : "memory");
       }
+      more = item_of<ROLE>(a, cluster, clusters, tile + 1, next);
+      if (more) ask(ahead, next);
+      const long long y = row < a.rows ? now.y : -1;
+      const bool live = ROLE == kDz && row < a.rows && y != a.ignore;
+      const float ref = now.ref, inv = now.inv, g = y >= 0 && y < a.all_classes ? now.up * unit : CUDART_NAN_F;  // of a live row
       // the row's own class as a column of this warp, -1: elsewhere
       const long long far = y - a.class0 - col_base;
       const int own = far >= 0 && far < kWide ? (int)far : -1;
@@ -688,7 +711,6 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         }
       } else {
         const Product& p = it.product ? a.dx : a.dw;
-        const float back = upstream_back(a.up);
         float* acc = p.acc ? p.acc + (p.splits > 1 ? (long long)it.split * p.M * p.N : 0) : nullptr;
         const bool out16 = PIECES == 1 && p.out;  // 16-bit results; else fp32, to the gradient or to the sums
         float* to32 = p.out ? (float*)p.out : acc;
