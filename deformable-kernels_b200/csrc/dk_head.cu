@@ -484,6 +484,7 @@ bool dtype_ok(int d) { return d == DK_F32 || d == DK_F16 || d == DK_BF16 || d ==
 bool options_ok(int reduction, double smoothing) {
   return reduction >= DK_REDUCE_NONE && reduction <= DK_REDUCE_SUM && smoothing >= 0.0 && smoothing <= 1.0;
 }
+// the kernels store 16 bytes at a time into the workspace as well
 bool aligned16(const void* a, const void* b) { return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0; }
 
 }  // namespace
@@ -503,7 +504,7 @@ int dk_linear_cross_entropy_forward(const void* input, const void* weight, const
                                     void* saved, int rows, int features, int classes, long long ignore_index, int reduction,
                                     double label_smoothing, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   if (!input || !weight || !target || !loss || !head::shape_ok(rows, features, classes) || !head::dtype_ok(dtype) ||
-      !head::options_ok(reduction, label_smoothing) || !head::aligned16(input, weight))
+      !head::options_ok(reduction, label_smoothing) || !head::aligned16(input, weight) || !head::aligned16(workspace, nullptr))
     return DK_ERR_BAD_ARGUMENT;
   const head::Shape h = {rows, features, classes, ignore_index, reduction, label_smoothing};
   cudaStream_t s = (cudaStream_t)stream;
@@ -523,7 +524,8 @@ int dk_linear_cross_entropy_backward(const void* grad_loss, const void* input, c
                                      void* grad_bias, int rows, int features, int classes, long long ignore_index, int reduction,
                                      double label_smoothing, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   if (!grad_loss || !input || !weight || !target || !saved || !head::shape_ok(rows, features, classes) || !head::dtype_ok(dtype) ||
-      !head::options_ok(reduction, label_smoothing) || !head::aligned16(input, weight) || !head::aligned16(grad_input, grad_weight))
+      !head::options_ok(reduction, label_smoothing) || !head::aligned16(input, weight) || !head::aligned16(grad_input, grad_weight) ||
+      !head::aligned16(workspace, nullptr))
     return DK_ERR_BAD_ARGUMENT;
   if (!grad_input && !grad_weight && !grad_bias) return DK_OK;
   const head::Shape h = {rows, features, classes, ignore_index, reduction, label_smoothing};

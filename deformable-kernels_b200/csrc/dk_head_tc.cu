@@ -184,9 +184,22 @@ __device__ __forceinline__ bool try_wait(unsigned bar, unsigned parity) {
       : "memory");
   return ok != 0;
 }
+__device__ __forceinline__ unsigned long long nanoseconds() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
+  return t;
+}
+// Two seconds: the longest sum a tile can have (2^27 values of dz in one piece, 65536 steps for a tile 32 wide) takes some 20 ms.
 __device__ __forceinline__ bool wait(unsigned bar, unsigned parity, volatile int* abort_flag) {
   bool done = try_wait(bar, parity);
-  for (unsigned i = 0; !done && i < ring::kMaxPolls && !*abort_flag; ++i) done = try_wait(bar, parity);
+  if (!done) {
+    const unsigned long long start = nanoseconds();
+    for (unsigned i = 1; !done && !*abort_flag; ++i) {
+      done = try_wait(bar, parity);
+      if ((i & 63) == 0 && nanoseconds() - start > 2000000000ull) break;
+      if (i == 1u << 30) break;
+    }
+  }
   if (!done) *abort_flag = 1;
   return __any_sync(0xffffffffu, *abort_flag != 0);
 }

@@ -13,48 +13,23 @@ __all__ = ['Dropout', 'LinearCrossEntropy']
 
 
 class Dropout(nn.Module):
-    """``nn.Dropout`` without a stored mask.  Each call in training mode draws from the next offset of the module's own
-    generator state ``[seed, offset]``, which lives on the device and advances there: a captured call draws anew at every
-    replay.  ``seed=None`` takes one from torch's default generator when the module is built.  ``shared_dims``: the
-    elements of that many trailing dimensions are dropped together (2: whole feature planes)."""
+    """``nn.Dropout`` without a stored mask.  Each call in training mode draws its generator's seed and offset on the device
+    from torch's default CUDA generator: ``torch.manual_seed`` repeats the masks, activation checkpointing makes the same
+    one again, and a captured call draws anew at every replay.  ``shared_dims``: the elements of that many trailing
+    dimensions are dropped together (2: whole feature planes)."""
 
-    def __init__(self, p=0.5, shared_dims=0, seed=None):
+    def __init__(self, p=0.5, shared_dims=0):
         super().__init__()
         if not 0 <= p <= 1:
             raise ValueError('dropout probability has to be between 0 and 1, but got {}'.format(p))
         self.p = p
         self.shared_dims = shared_dims
-        self.seed = int(torch.randint(0, 2 ** 62, ())) if seed is None else seed
-        # not a buffer: data-parallel wrappers would make every rank's state that of rank 0
-        self._state = self._step = None
-
-    def rng_state(self):
-        """[seed, offset of the next call]: what set_rng_state takes to go on from here."""
-        return [self.seed, 0] if self._state is None else self._state.tolist()
-
-    def set_rng_state(self, state):
-        self.seed, offset = state
-        if self._state is not None:
-            self._state.copy_(torch.tensor([self.seed, offset]))
-        else:
-            self._start = offset
-
-    _start = 0
-
-    def _state_on(self, device):
-        if self._state is None or self._state.device != device:
-            offset = self._start if self._state is None else int(self._state[1])
-            self._state = torch.tensor([self.seed, offset], device=device)
-            self._step = torch.tensor([0, 1], device=device)
-        return self._state
 
     def forward(self, input):
         if not self.training or self.p == 0:
             return input
-        state = self._state_on(input.device)
-        out = dropout(input, self.p, state, shared_dims=self.shared_dims)
-        state.add_(self._step)
-        return out
+        state = torch.randint(0, 2 ** 63 - 1, (2,), device=input.device)
+        return dropout(input, self.p, state, shared_dims=self.shared_dims)
 
     def extra_repr(self):
         return 'p={}, shared_dims={}'.format(self.p, self.shared_dims)

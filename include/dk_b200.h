@@ -303,8 +303,8 @@ int dk_dropout(const void *input, void *output, long long count, long long run, 
  * target outside [0, classes) gives NaN.  reduction: DK_REDUCE_MEAN divides by the number of rows that count (none: the
  * loss is NaN, the gradients are zero).  loss: one value, or [rows] for DK_REDUCE_NONE; it, `saved` and grad_loss are
  * float (double for DK_F64).  saved: 2 rows + 2 values that the backward takes back, or
- * NULL.  input, weight and
- * their gradients begin on 16 bytes.  Any gradient may be NULL. */
+ * NULL.  input, weight,
+ * their gradients and the workspace begin on 16 bytes.  Any gradient may be NULL. */
 typedef enum dk_reduction { DK_REDUCE_NONE = 0, DK_REDUCE_MEAN = 1, DK_REDUCE_SUM = 2 } dk_reduction;
 size_t dk_linear_cross_entropy_forward_workspace_bytes(int rows, int features, int classes, int dtype);
 int dk_linear_cross_entropy_forward(const void *input, const void *weight, const void *bias, const long long *target,

@@ -83,6 +83,7 @@ def test_library_refuses_bad_calls_before_any_launch():
     for bad in (dict(x=null), dict(w=null), dict(y=null), dict(loss=null), dict(rows=0), dict(features=0), dict(classes=0), dict(reduction=3),
                 dict(reduction=-1), dict(smoothing=-0.1), dict(smoothing=1.5), dict(smoothing=float("nan")), dict(dtype=4)):
         assert forward(**bad) == 1, bad
+    assert forward(x=ctypes.c_void_p(24)) == 1 and forward(ws=ctypes.c_void_p(24), size=1 << 30) == 1
     assert forward() == 3 and forward(ws=one, size=16) == 3                                   # no workspace, too little
 
     def backward(up=one, saved=one, dtype=0, ws=null, size=0, rows=2):
@@ -112,10 +113,8 @@ def test_modules_have_the_stock_parameters():
     head.eval()
     assert torch.equal(head(x), stock(x))                        # logits need no kernel of ours
     assert "label_smoothing=0.1" in repr(head)
-    d = Dropout(0.3, shared_dims=2, seed=7)
+    d = Dropout(0.3, shared_dims=2)
     assert d.eval()(x) is x and Dropout(0.0)(x) is x
-    assert d.rng_state() == [7, 0]
-    d.set_rng_state([9, 4])
-    assert d.seed == 9 and d._start == 4
+    assert not list(d.state_dict()) and not list(d.buffers())
     with pytest.raises(ValueError):
         Dropout(1.5)

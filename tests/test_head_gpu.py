@@ -1,6 +1,7 @@
 """The classifier head on the GPU: dropout bit by bit, the loss and its gradients within derived bounds."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import head_oracle as H
 
@@ -77,23 +78,58 @@ def test_dropout_state_on_the_device_and_replayed_graphs():
     dx, = torch.autograd.grad(y, xg, x)
     assert torch.equal(y.detach().cpu(), want[0]) and torch.equal(dx.cpu(), want[0])
 
-    from deformable_kernels.modules import Dropout
-    m = Dropout(0.4, seed=99)
+    # captured: what the tensor holds at each replay
+    state.copy_(torch.tensor([99, 10]))
     xs = x.clone().requires_grad_(True)
-    side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(side):
-        torch.autograd.grad(m(xs), xs, x)
-    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = functions().dropout(xs, 0.4, state)
+        state[1] += 1
+        dx, = torch.autograd.grad(y, xs, x)
+    for i in range(3):
+        g.replay()
+        assert torch.equal(y.detach().cpu(), want[i]) and torch.equal(dx.cpu(), want[i])
+
+
+def test_dropout_module_draws_from_torchs_generator():
+    from deformable_kernels.modules import Dropout
+    m = Dropout(0.4, shared_dims=1)
+    x = torch.randn(200, 3, device=DEV)
+
+    def run(seed, f=m):
+        torch.manual_seed(seed)
+        xs = x.clone().requires_grad_(True)
+        y = f(xs)
+        return y.detach(), torch.autograd.grad(y, xs, x)[0]
+    (a, ga), (b, gb), (c, _) = run(5), run(5), run(6)
+    assert torch.equal(a, b) and torch.equal(ga, gb) and torch.equal(a, ga) and not torch.equal(a, c)
+    # a checkpointed call makes the same mask again for its backward
+    d, gd = run(5, lambda t: torch.utils.checkpoint.checkpoint(m, t, use_reentrant=False))
+    assert torch.equal(a, d) and torch.equal(a, gd)
+    # replays draw anew, and their backwards what they drew
+    xs = x.clone().requires_grad_(True)
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         y = m(xs)
         dx, = torch.autograd.grad(y, xs, x)
-    m.set_rng_state([99, 10])
-    for i in range(3):
+    seen = []
+    for _ in range(3):
         g.replay()
-        assert torch.equal(y.detach().cpu(), want[i]) and torch.equal(dx.cpu(), want[i])
-    assert m.rng_state() == [99, 13]
+        assert torch.equal(y, dx)
+        seen.append(y.detach().clone())
+    assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
+def test_dropout_beyond_32_bits():
+    """2^33 + 24 elements: the index of a draw and the offsets of elements pass 32 bits, the launch is split."""
+    n = 2 ** 33 + 24
+    x = torch.ones(n, device=DEV, dtype=torch.float16)
+    y = functions().dropout(x, 0.3, 11, 2 ** 35 + 1)
+    index = torch.cat([torch.arange(64), torch.arange(2 ** 32 - 32, 2 ** 32 + 32), torch.arange(2 ** 33 - 32, n)])
+    keep = torch.from_numpy(H.draws(index.numpy(), 11, 2 ** 35 + 1).astype("int64")) >= int(0.3 * 2 ** 32 + 0.5)
+    assert torch.equal(y[index.to(DEV)].cpu() != 0, keep)
+    del x, y
+    torch.cuda.empty_cache()
 
 
 def test_dropout_refusals():
@@ -399,16 +435,18 @@ def test_head_and_dropout_together_as_a_training_step():
     torch.manual_seed(5)
     x, w, y, b, up = make(90, 56, 120, "fp32", seed=15)
     head = LinearCrossEntropy(56, 120, dropout=0.25, label_smoothing=0.1).to(DEV)
-    head.dropout.set_rng_state([41, 3])
     with torch.no_grad():
         head.weight.copy_(w), head.bias.copy_(b)
     for step in range(3):
+        torch.manual_seed(step)
+        seed, offset = torch.randint(0, 2 ** 63 - 1, (2,), device=DEV).tolist()
+        torch.manual_seed(step)
         xg = x.to(DEV).requires_grad_(True)
         loss = head(xg, y.to(DEV))
         dx, dw, db = torch.autograd.grad(loss, [xg, head.weight, head.bias])
-        dropped = H.dropout(x, 0.25, 41, 3 + step)
+        dropped = H.dropout(x, 0.25, seed, offset)
         out, far = H.head(dropped, w, y, b, torch.tensor(1.0), label_smoothing=0.1)
-        keep = H.keep_mask(x.shape, 0.25, 41, 3 + step).double() / 0.75
+        keep = H.keep_mask(x.shape, 0.25, seed, offset).double() / 0.75
         out["dx"], far["dx"] = out["dx"] * keep, far["dx"] * keep + out["dx"].abs() * 2.0 ** -22 + 1e-300
         for name, v in (("loss", loss), ("dx", dx), ("dw", dw), ("db", db)):
             assert ((v.detach().cpu().double() - out[name]).abs() <= far[name]).all(), (step, name)
@@ -433,6 +471,7 @@ def test_calls_from_threads_that_have_not_used_the_gpu_yet():
 import sys, threading
 sys.path[:0] = [%r, %r]
 import torch
+import torch.utils.checkpoint
 import head_oracle as H
 import test_head_gpu as T
 cases = [T.make(60, 32, 50, "bf16", seed=s) for s in range(4)]
@@ -453,6 +492,49 @@ assert not wrong, wrong
 """ % (os.path.join(root, "deformable-kernels_b200"), os.path.join(root, "tests"))
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
     assert out.returncode == 0, out.stderr[-2000:]
+
+
+def test_features_and_weights_beyond_32_bits():
+    """More than 2^32 features or weights: what is far behind is what a call on those rows or classes alone gives."""
+    f = functions()
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    t, d, v = 2 ** 21 + 5, 2056, 24
+    x = torch.randn(t, d, device=DEV, generator=gen, dtype=torch.bfloat16)
+    w = torch.randn(v, d, device=DEV, generator=gen, dtype=torch.bfloat16) / 32
+    y = torch.randint(0, v, (t,), device=DEV, generator=gen)
+    x.requires_grad_(True)
+    loss = f.linear_cross_entropy(x, w, y, reduction="none")
+    dx, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    loss = loss.detach()
+    for lo in (0, 2 ** 20 - 100, t - 300):
+        part = x.detach()[lo:lo + 300].clone().requires_grad_(True)
+        want = f.linear_cross_entropy(part, w, y[lo:lo + 300], reduction="none")
+        dpart, = torch.autograd.grad(want, part, torch.ones_like(want))
+        # the same products in another tiling: 2056 cutting additions of 2^-23 each at most, a rounding of dz and of dx that may fall to the
+        # other side (2^-7 of the value, 2^-8 of every class's part)
+        assert (loss[lo:lo + 300] - want.detach()).abs().max() < 1e-3
+        assert (dx[lo:lo + 300].float() - dpart.float()).abs().max() < 2.0 ** -6 * w.float().abs().max()
+    del x, dx, loss
+    torch.cuda.empty_cache()
+    t, v = 40, 2 ** 21 + 5
+    x = torch.randn(t, d, device=DEV, generator=gen, dtype=torch.bfloat16)
+    w = (torch.randn(v, d, device=DEV, generator=gen, dtype=torch.bfloat16) / 32).requires_grad_(True)
+    y = torch.randint(0, v, (t,), device=DEV, generator=gen)
+    y[:4] = torch.tensor([0, 2 ** 20, v - 1, v - 2])
+    loss = f.linear_cross_entropy(x, w, y, reduction="none")
+    dw, = torch.autograd.grad(loss, w, torch.ones_like(loss))
+    z = torch.cat([x.float() @ w.detach()[i:i + 2 ** 18].float().t() for i in range(0, v, 2 ** 18)], 1)
+    lse = torch.logsumexp(z, 1)
+    assert (loss.detach() - (lse - z.gather(1, y[:, None]).squeeze(1))).abs().max() < 1e-2
+    for lo in (0, 2 ** 20 - 50, v - 100):
+        dz = torch.exp(z[:, lo:lo + 100] - lse[:, None])
+        hit = (y >= lo) & (y < lo + 100)
+        dz[hit, y[hit] - lo] -= 1
+        want = dz.t() @ x.float()
+        # dz and dw are rounded to bf16: 2^-8 of the magnitudes each; the logits' error moves p by a few 1e-3 of itself
+        assert ((dw[lo:lo + 100].float() - want).abs() <= 2.0 ** -6 * (dz.abs().t() @ x.float().abs()) + 1e-6).all()
+    del w, dw, z
+    torch.cuda.empty_cache()
 
 
 def test_training_step_of_the_bench_with_the_fused_head():
