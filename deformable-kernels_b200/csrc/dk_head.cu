@@ -319,19 +319,21 @@ template int launch_few_rows<float>(const void*, const void*, const void*, const
 
 // ------------------------------------------------------------------ the tiles of a row joined
 
-// A block has 32 rows; its warps share the slots.  partial: per block the sum of the losses, the rows that count, and whether an
-// ignored row's logits are not finite; the last block to finish joins those, in fixed order.
+// A block has `groups` times 32 rows; its other warps share the slots of those.  partial: per block the sum of the losses, the rows that
+// count, and whether an ignored row's logits are not finite; the last block to finish joins those, in fixed order.
 template <typename A>
-__global__ void __launch_bounds__(1024) combine_kernel(Partials<A> p, const long long* __restrict__ y, int slots, void* loss,
+__global__ void __launch_bounds__(1024) combine_kernel(Partials<A> p, const long long* __restrict__ y, int slots, int groups, void* loss,
                                                        A* saved, double* partial, unsigned* count, Shape h) {
-  __shared__ A s_top[32][33], s_sum[32][33], s_all[32][33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int r = blockIdx.x * 32 + lane;
+  __shared__ A s_top[32][33], s_sum[32][33], s_all[32][33];  // [warp][lane]
+  __shared__ double s_v[32][3];
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, share = warps / groups;
+  const int group = (threadIdx.x >> 5) / share, warp = (threadIdx.x >> 5) - group * share;
+  const int r = (blockIdx.x * groups + group) * 32 + lane;
   before_all();
   A top = minus_inf<A>(), sum = (A)0, all = (A)0;
   if (r < h.T) {
 #pragma unroll 4
-    for (int s = warp; s < slots; s += warps) {
+    for (int s = warp; s < slots; s += share) {
       const long long at = (long long)s * h.T + r;
       const A t = p.top[at], n = fmax(top, t), ref = n == minus_inf<A>() ? (A)0 : n;
       sum = sum * power(top - ref) + p.sum[at] * power(t - ref);
@@ -339,19 +341,23 @@ __global__ void __launch_bounds__(1024) combine_kernel(Partials<A> p, const long
       if (h.smoothing != 0.0) all += p.all[at];
     }
   }
-  s_top[lane][warp] = top, s_sum[lane][warp] = sum, s_all[lane][warp] = all;
-  __syncthreads();
-  if (warp) return;
-  A most = minus_inf<A>();
+  if (share > 1) {
+    s_top[threadIdx.x >> 5][lane] = top, s_sum[threadIdx.x >> 5][lane] = sum, s_all[threadIdx.x >> 5][lane] = all;
+    __syncthreads();
+  }
+  A ref = top == minus_inf<A>() ? (A)0 : top;
+  if (warp == 0 && share > 1) {
+    const int first = group * share;
 #pragma unroll 8
-  for (int i = 0; i < warps; ++i) most = fmax(most, s_top[lane][i]);
-  const A ref = most == minus_inf<A>() ? (A)0 : most;
-  sum = all = (A)0;
+    for (int i = 1; i < share; ++i) top = fmax(top, s_top[first + i][lane]);
+    ref = top == minus_inf<A>() ? (A)0 : top;
+    sum = all = (A)0;
 #pragma unroll 8
-  for (int i = 0; i < warps; ++i) sum += s_sum[lane][i] * power(s_top[lane][i] - ref), all += s_all[lane][i];
+    for (int i = 0; i < share; ++i) sum += s_sum[first + i][lane] * power(s_top[first + i][lane] - ref), all += s_all[first + i][lane];
+  }
   const A ls = log(sum);
   double v[3] = {0, 0, 0};  // loss, rows that count, ignored rows that are not finite
-  if (r < h.T) {
+  if (warp == 0 && r < h.T) {
     const long long yr = y[r];
     A one = (A)0;
     if (yr != h.ignore) {
@@ -368,21 +374,31 @@ __global__ void __launch_bounds__(1024) combine_kernel(Partials<A> p, const long
     if (saved) saved[r] = ref, saved[h.T + r] = (A)1 / sum;
   }
   if (!saved && h.reduction == DK_REDUCE_NONE) return;
-  for (int k = 0; k < 3; ++k)
+  if (warp == 0) {
+    for (int k = 0; k < 3; ++k)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+      for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    if (lane == 0)
+      for (int k = 0; k < 3; ++k) s_v[group][k] = v[k];
+  }
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  v[0] = v[1] = v[2] = 0;
+  for (int g = 0; g < groups; ++g)
+    for (int k = 0; k < 3; ++k) v[k] += s_v[g][k];
   if (gridDim.x > 1) {
     unsigned turn = 0;
     if (lane == 0) {
-      for (int k = 0; k < 3; ++k) partial[3 * blockIdx.x + k] = v[k];
+      for (int k = 0; k < 3; ++k) partial[3ll * blockIdx.x + k] = v[k];
       __threadfence();
       turn = atomicAdd(count, 1u);
     }
     if (__shfl_sync(0xffffffffu, turn, 0) != gridDim.x - 1) return;
     __threadfence();
     v[0] = v[1] = v[2] = 0;
+#pragma unroll 4
     for (unsigned i = lane; i < gridDim.x; i += 32)
-      for (int k = 0; k < 3; ++k) v[k] += __ldcg(partial + 3 * i + k);
+      for (int k = 0; k < 3; ++k) v[k] += __ldcg(partial + 3ll * i + k);
     for (int k = 0; k < 3; ++k)
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
@@ -395,10 +411,13 @@ __global__ void __launch_bounds__(1024) combine_kernel(Partials<A> p, const long
 template <typename A>
 int launch_combine(const Partials<A>& p, const long long* y, int slots, void* loss, void* saved, double* partial, const Shape& h,
                    cudaStream_t s) {
-  int warps = 1;  // four slots a warp
-  while (warps < 32 && warps * 4 < slots) warps *= 2;
-  return launch_after(combine_kernel<A>, div_up(h.T, kCombineRows), 32 * warps, 0, 1, s, p, y, slots, loss, (A*)saved, partial,
-                      combine_count(partial, h.T), h);
+  int share = 1;  // four slots a warp
+  while (share < 32 && share * 4 < slots) share *= 2;
+  // as many rows a block as leave every SM one: fewer blocks to join
+  int groups = 1;
+  while (groups * 2 * share <= 32 && div_up(h.T, 64 * groups) >= device_sm_count()) groups *= 2;
+  return launch_after(combine_kernel<A>, div_up(h.T, kCombineRows * groups), 32 * share * groups, 0, 1, s, p, y, slots, groups, loss, (A*)saved,
+                      partial, combine_count(partial, h.T), h);
 }
 template int launch_combine<float>(const Partials<float>&, const long long*, int, void*, void*, double*, const Shape&, cudaStream_t);
 

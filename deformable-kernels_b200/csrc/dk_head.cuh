@@ -77,7 +77,7 @@ __device__ __forceinline__ A upstream_back(const Upstream<A>& u) {
 }
 
 // ---- the slots of a row joined (dk_head.cu)
-constexpr int kCombineRows = 32;  // rows of a block
+constexpr int kCombineRows = 32;  // rows of a block, or a multiple
 // sums of the blocks, and the count of those that are done, which the kernel before sets to zero
 inline size_t combine_bytes(int T) { return (size_t)div_up(T, kCombineRows) * 3 * sizeof(double) + sizeof(double); }
 // losses, log-sum-exps and counts; `partial`: combine_bytes(), the count last

@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           float z[32];
           columns(z, c0);
           const float4* bp = reinterpret_cast<const float4*>(bias + grp * kWide + c0);
-          float most = -CUDART_INF_F;
+          float most[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             const float4 v = bp[q];
@@ -642,12 +642,15 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           }
           if (a.all) {
             const int in = a.classes - col_base - c0;
+            float some[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) all += j < in ? z[j] : 0.0f;
+            for (int j = 0; j < 32; ++j) some[j & 3] += j < in ? z[j] : 0.0f;
+            all += (some[0] + some[1]) + (some[2] + some[3]);
           }
+          // chains of eight: four at a time
 #pragma unroll
-          for (int j = 0; j < 32; ++j) most = fmaxf(most, z[j]);
-          const float n = fmaxf(top, most), ref = n == -CUDART_INF_F ? 0.0f : n;
+          for (int j = 0; j < 32; ++j) most[j & 3] = fmaxf(most[j & 3], z[j]);
+          const float n = fmaxf(top, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))), ref = n == -CUDART_INF_F ? 0.0f : n;
           float part[4] = {0, 0, 0, 0};
 #pragma unroll
           for (int j = 0; j < 32; ++j) part[j & 3] += ex2((z[j] - ref) * kL2);
@@ -728,6 +731,33 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         const bool out16 = PIECES == 1 && p.out;  // 16-bit results; else fp32, to the gradient or to the sums
         float* to32 = p.out ? (float*)p.out : acc;
         const bool vec = (p.N & (out16 ? 7 : 3)) == 0;
+        if (PIECES == 1 && out16 && vec && p.first) {
+          // the result at once: packed before the staging, 16 bytes a lane and eight lanes a row behind it
+#pragma unroll 1
+          for (int c0 = 0; c0 < kWide; c0 += kBox) {
+            if (row_base >= p.M || col_base + c0 >= p.N) break;  // of the whole warp
+            float v[2][32];
+            __syncwarp();
+            ld32(v[0], d + c0);
+            ld32(v[1], d + c0 + 32);
+            wait_ld(v[0]);
+            wait_ld(v[1]);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const float* f = &v[q >> 2][(q & 3) * 8];
+              sts16(staged(stage, lane, q), pack<E>(f[0] * back, f[1] * back), pack<E>(f[2] * back, f[3] * back),
+                    pack<E>(f[4] * back, f[5] * back), pack<E>(f[6] * back, f[7] * back));
+            }
+            __syncwarp();
+            const int c = col_base + c0 + 8 * (lane & 7);
+            E* to = (E*)p.out + (long long)(row_base + (lane >> 3)) * p.N + c;
+#pragma unroll
+            for (int r = 0; r < 32; r += 4, to += 4ll * p.N)
+              if (row_base + r + (lane >> 3) < p.M && c < p.N) *reinterpret_cast<uint4*>(to) = lds16(staged(stage, r + (lane >> 3), lane & 7));
+          }
+          release(b);
+          continue;
+        }
 #pragma unroll(PIECES == 1 ? 1 : 2)
         for (int c0 = 0; c0 < kWide; c0 += 32) {
           if (row_base >= p.M || col_base + c0 >= p.N) break;  // of the whole warp
@@ -979,12 +1009,15 @@ void split_products(BackwardPlan& p, int D, int pieces) {
 }
 
 // the rounds of the two products' items that let all clusters end at about the same time
-Schedule schedule_of(const Product& dw, const Product& dx, int clusters) {
+Schedule schedule_of(const Product& dw, const Product& dx, int clusters, int pieces) {
+  // a tile takes the epilogue as long as it takes the tensor cores ten steps (six products a step: two)
+  const int least = pieces == 1 ? 10 : 2;
   const int n_w = dw.tiles_m * dw.tiles_n * dw.splits, n_x = dx.tiles_m * dx.tiles_n * dx.splits;
   Schedule c = {};
   c.long_product = n_w == 0 || (n_x != 0 && dx.per > dw.per);
   c.n_long = c.long_product ? n_x : n_w, c.n_short = c.long_product ? n_w : n_x;
-  const long long per_long = c.long_product ? dx.per : dw.per, per_short = c.long_product ? dw.per : dx.per;
+  long long per_long = c.long_product ? dx.per : dw.per, per_short = c.long_product ? dw.per : dx.per;
+  per_long = per_long < least ? least : per_long, per_short = per_short < least ? least : per_short;
   const int rest = c.n_long % clusters;
   long long dealt = 0;
   while (dealt < c.n_short) {
@@ -1169,7 +1202,7 @@ int backward(const void* up, const void* x, const void* w, const void* b, const 
           px.acc = (float*)(m + p.parts_x), px.out = nullptr, px.first = 1;
         }
       }
-      a.dw = pw, a.dx = px, a.schedule = schedule_of(pw, px, clusters_of(p.grad));
+      a.dw = pw, a.dx = px, a.schedule = schedule_of(pw, px, clusters_of(p.grad), PIECES);
       if (db) a.acc_b = cut_v ? nullptr : (float*)(m + p.acc_b), a.out_b = last_t ? (T*)db + v0 : nullptr, a.first_b = first_t;
       const long long items = (long long)pw.tiles_m * tn * pw.splits + (long long)px.tiles_m * tn * px.splits;
       if (items > 0x3fffffff) return DK_ERR_UNSUPPORTED;
