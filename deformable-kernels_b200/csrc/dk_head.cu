@@ -378,14 +378,16 @@ __global__ void __launch_bounds__(1024) combine_kernel(Partials<A> p, const long
     for (int k = 0; k < 3; ++k)
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-    if (lane == 0)
+    if (lane == 0 && groups > 1)
       for (int k = 0; k < 3; ++k) s_v[group][k] = v[k];
   }
-  __syncthreads();
+  if (groups > 1) __syncthreads();
   if (threadIdx.x >= 32) return;
-  v[0] = v[1] = v[2] = 0;
-  for (int g = 0; g < groups; ++g)
-    for (int k = 0; k < 3; ++k) v[k] += s_v[g][k];
+  if (groups > 1) {
+    v[0] = v[1] = v[2] = 0;
+    for (int g = 0; g < groups; ++g)
+      for (int k = 0; k < 3; ++k) v[k] += s_v[g][k];
+  }
   if (gridDim.x > 1) {
     unsigned turn = 0;
     if (lane == 0) {
