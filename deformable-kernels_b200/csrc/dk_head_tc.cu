@@ -12,6 +12,13 @@
 // pieces that reach 2^-24 are taken from three stages, that of the leading pieces into one accumulator, the five
 // small ones into another: the additions of the tensor cores cut, and a cut of the small sum costs nothing.  After every eight steps
 // the epilogue adds both to sums in registers, which round, so that no more than 32 cuts meet in one value.
+//
+// Measured, one B200: logits with statistics 1.29 ms at 8192 x 2048 x 65536 (2.20 Tflop: 1.71 Pflop/s, tensor pipe 96 % of the
+// cycles), 0.146 at 4096 x 1280 x 21841 (1.57 Pflop/s, 87 %: 19 rounds of tiles, the last a half); with dz 0.174 (70 %: its 179 MB
+// contend with the loads in L2, 10 TB/s of them; without the stores 88 % of the cycles); the two products 0.313
+// (1.46 Pflop/s, 83 %).  The clock is at 1.5 GHz under this load: power is the bound of large calls.
+// Small calls are launches and the latency of one tile: 10 us for a tile of 1280 features.
+
 #include <math_constants.h>
 
 #include <type_traits>
