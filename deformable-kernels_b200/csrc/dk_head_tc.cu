@@ -478,6 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
     }
   } else if (warp == 1) {
     // ---------------- mma, the leading block only
+    before_all();  // it reads nothing, but its waits are not to run while the kernel before does
     if (rank == 0) {
       const bool one = tc::elect_one();
       constexpr unsigned kDesc = (1u << 4) | type_bits<E>() | ((unsigned)(BN >> 3) << 17) | ((unsigned)(128 * CG >> 4) << 24);
@@ -1085,9 +1086,9 @@ unsigned blocks_for(long long n) {
 }
 
 // tiles of rows whose part of x stays in L2 (126 MB) beside the weights that stream past
-int row_group(const Config& c, int D, int pieces) {
+int row_group(const Config& c, int D, int pieces, int tiles_m) {
   const long long g = (40ll << 20) / ((long long)128 * c.cg * D * 2 * pieces);
-  return g < 1 ? 1 : (int)(g > 1 << 20 ? 1 << 20 : g);
+  return g < 1 ? 1 : (int)(g > tiles_m ? tiles_m : g);
 }
 
 // x and w as planes of 16-bit values that TMA can fetch
@@ -1124,7 +1125,7 @@ int forward(const void* x, const void* w, const void* b, const long long* y, voi
   if (!operand_map<E, PIECES>(&a.x, x, h.T, h.D, pitch_of(h.D)) || !operand_map<E, PIECES>(&a.w, w, h.V, h.D, pitch_of(h.D)))
     return DK_ERR_CUDA;
   a.rows = h.T, a.classes = h.V, a.depth = div_up(h.D, kBox);
-  a.tiles_m = p.tiles_m, a.tiles_n = p.tiles_n, a.group = row_group(p.c, h.D, PIECES);
+  a.tiles_m = p.tiles_m, a.tiles_n = p.tiles_n, a.group = row_group(p.c, h.D, PIECES, p.tiles_m);
   a.bias = b, a.target = y, a.ignore = h.ignore;
   a.top = (float*)(m + p.top), a.sum = (float*)(m + p.sum), a.all = h.smoothing != 0.0 ? (float*)(m + p.all) : nullptr;
   a.picked = (float*)(m + p.picked), a.done = combine_count((double*)(m + p.partial), h.T);
@@ -1175,11 +1176,12 @@ int backward(const void* up, const void* x, const void* w, const void* b, const 
           !operand_map<E, PIECES>(&a.dz_out, m + p.buffer, rows, classes, dz_pitch, 32))
         return DK_ERR_CUDA;
       a.rows = rows, a.classes = classes, a.row0 = t0, a.class0 = v0;
-      a.tiles_m = div_up(rows, 128 * p.dz.cg), a.tiles_n = div_up(classes, p.dz.bn), a.group = row_group(p.dz, h.D, PIECES);
+      a.tiles_m = div_up(rows, 128 * p.dz.cg), a.tiles_n = div_up(classes, p.dz.bn), a.group = row_group(p.dz, h.D, PIECES, a.tiles_m);
       a.target = y + t0, a.ref = stat + t0, a.inv = stat + h.T + t0;
       if (h.reduction == DK_REDUCE_NONE) a.up.up = (const float*)up + t0;
       if (a.strange && first_t && first_v) a.dirty = x, a.clean = m + p.x, a.width = h.D, a.up_rows = h.T, a.target_all = y;
       else a.clean = nullptr;
+      if ((long long)a.tiles_m * a.tiles_n > 0x3fffffff) return DK_ERR_UNSUPPORTED;
       rc = launch<kDz, E, PIECES>(p.dz, a, a.tiles_m * a.tiles_n, s);
       if (rc != DK_OK) return rc;
       // dw [classes][D] sums over rows, dx [rows][D] over classes; the running sums of fp32 gradients are the gradients
@@ -1209,10 +1211,10 @@ int backward(const void* up, const void* x, const void* w, const void* b, const 
           px.acc = (float*)(m + p.parts_x), px.out = nullptr, px.first = 1;
         }
       }
-      a.dw = pw, a.dx = px, a.schedule = schedule_of(pw, px, clusters_of(p.grad), PIECES);
       if (db) a.acc_b = cut_v ? nullptr : (float*)(m + p.acc_b), a.out_b = last_t ? (T*)db + v0 : nullptr, a.first_b = first_t;
       const long long items = (long long)pw.tiles_m * tn * pw.splits + (long long)px.tiles_m * tn * px.splits;
       if (items > 0x3fffffff) return DK_ERR_UNSUPPORTED;
+      a.dw = pw, a.dx = px, a.schedule = schedule_of(pw, px, clusters_of(p.grad), PIECES);
       rc = launch<kGrad, E, PIECES>(p.grad, a, (int)items, s);
       if (rc == DK_OK && jw.count + jx.count > 0) rc = launch_after(join_kernel<T>, blocks_for(jw.count + jx.count), 256, 0, 1, s, jw, jx);
       if (rc != DK_OK) return rc;

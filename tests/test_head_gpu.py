@@ -429,6 +429,55 @@ def test_head_on_another_stream_and_captured():
             assert all(torch.equal(a, c) for a, c in zip(want, out))
 
 
+def test_two_streams_at_once():
+    """Calls of different sizes on two streams, none waiting for the other: each has its own scratch, and what is on the
+    chip of an SM belongs to one block at a time."""
+    f = functions()
+    cases = [make(3000, 264, 5000, "bf16", seed=21), make(40, 64, 300, "fp32", seed=22)]
+    streams = [torch.cuda.Stream() for _ in cases]
+
+    def step(case):
+        x, w, y, b, up = (t.to(DEV) for t in case)
+        leaves = [t.requires_grad_(True) for t in (x, w, b)]
+        loss = f.linear_cross_entropy(x, w, y, b)
+        return (loss.detach(),) + torch.autograd.grad(loss, leaves, up)
+    want = [step(c) for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, c) for a, c in zip(want[i], g))
+
+
+def test_gradients_that_arrive_expanded_or_in_another_dtype():
+    x, w, y, b, _ = make(50, 40, 60, "fp16", reduction="none", seed=30)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    loss = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), leaves[2], reduction="none")
+    want = torch.autograd.grad(loss, leaves, torch.ones(50, device=DEV), retain_graph=True)
+    for got in (torch.autograd.grad(loss.sum(), leaves, retain_graph=True), torch.autograd.grad(loss.double().sum(), leaves, retain_graph=True),
+                torch.autograd.grad(loss, leaves, torch.ones(1, device=DEV).expand(50))):
+        assert all(torch.equal(a, c) for a, c in zip(want, got))
+
+
+def test_gradients_of_broadcast_inputs_and_shared_weights():
+    """One feature row for many targets, one weight in two losses: autograd sums what the operator gives for each."""
+    f = functions()
+    x, w, y, b, _ = (t.to(DEV) for t in make(30, 24, 40, "fp64", seed=31))
+    one = x[:1].clone().requires_grad_(True)
+    wp = w.clone().requires_grad_(True)
+    loss = f.linear_cross_entropy(one.expand(30, 24), wp, y, b) + f.linear_cross_entropy(x, wp, y.flip(0), b, label_smoothing=0.2)
+    got = torch.autograd.grad(loss, [one, wp])
+    want = torch.nn.functional.cross_entropy(one.expand(30, 24) @ wp.t() + b, y) + \
+        torch.nn.functional.cross_entropy(x @ wp.t() + b, y.flip(0), label_smoothing=0.2)
+    for a, c in zip(got, torch.autograd.grad(want, [one, wp])):
+        assert torch.allclose(a, c, rtol=1e-11, atol=1e-13)
+
+
 def test_head_and_dropout_together_as_a_training_step():
     """Features -> dropout -> linear -> loss, as the module runs it, against the oracles one after the other."""
     from deformable_kernels.modules import LinearCrossEntropy
