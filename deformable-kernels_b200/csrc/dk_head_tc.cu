@@ -933,13 +933,29 @@ __global__ void __launch_bounds__(256) join_kernel(const Join a, const Join b) {
 struct Config {
   int cg, bn;
 };
-// Two SMs a tile where their tiles keep half of the pairs busy; below that tiles of one SM, narrow ones when even the wide
-// leave half of the SMs without one.
-Config pick(long long rows, long long cols, int pieces) {
-  const int sms = device_sm_count(), wide = pieces == 1 ? 256 : 128;  // two accumulators of fp32 pieces: half the columns
-  if ((long long)div_up(rows, 256) * div_up(cols, wide) * 4 >= sms) return {2, wide};
-  if ((long long)div_up(rows, 128) * div_up(cols, 128) * 2 >= sms) return {1, 128};
-  return {1, 64};
+// Tiles of the logits (us of the loss as a CUDA graph, 1280 features; pairs / 128 wide / 64 wide).  Pairs where one round of 128 x 128 tiles is not enough
+// (4096 rows, 1000 classes 19.4 / 22.3 / 32.0; 2048 rows 18.2 / 16.0 / 21.1), unless half of their rows would be empty (64 rows, 16384 classes 18.6 / 16.5 /
+// 22.2); narrow tiles while one round of them is (1024 rows, 1000 classes 17.5 / 15.0 / 14.5).  fp32: pairs also for fewer tiles when there are 16 steps or more,
+// whose loads they halve (256 rows, 1000 classes 30.3 / 34.4 / 32.0; of 256 features 16.0 / 15.5 / 14.9; 64 rows, 16384 classes 101 / 75 / 93).
+Config pick(long long rows, long long cols, int D, int pieces) {
+  const int sms = device_sm_count();
+  const long long tiles = (long long)div_up(rows, 128) * div_up(cols, 128);
+  if (rows > 128 && pieces == 1 && tiles > sms) return {2, 256};
+  if (rows > 128 && pieces == 3 && (tiles * 2 >= sms || div_up(D, kBox) >= 16)) return {2, 128};
+  return tiles * 2 >= sms ? Config{1, 128} : Config{1, 64};
+}
+// Tiles of the gradients (us of loss and gradients, as above).  Pairs where there is work for 27 steps of each (4096 rows, 16384 classes 465 / 600 / 867), or where
+// both sums are 16 steps long and a quarter of the SMs get a tile (1024 rows, 1000 classes 34.8 / 37.5 / 39.7); thin sums end sooner in tiles of one
+// SM (64 rows, 4096 classes 40.1 / 36.9 / 39.0; 512 rows 46.7 / 45.1 / 48.9), narrow ones while they are few (512 rows, 1000 classes of 256 features
+// 25.2 / 22.5 / 21.7).  fp32: pairs unless half of their rows would be empty (256 rows, 4096 classes 103 / 107 / 122; 64 rows 95 / 89 / 96).
+Config pick_gradients(long long rows, long long classes, int D, int pieces) {
+  const int sms = device_sm_count();
+  if (pieces == 3) return rows > 128 ? Config{2, 128} : Config{1, 128};
+  const long long row_tiles = div_up(rows, 256), class_tiles = div_up(classes, 256), n = div_up(D, 256);
+  const long long row_steps = div_up(rows, kBox), class_steps = div_up(classes, kBox);
+  if ((row_tiles * class_steps + class_tiles * row_steps) * n >= 27ll * (sms / 2)) return {2, 256};
+  if (row_steps >= 16 && class_steps >= 16 && (row_tiles + class_tiles) * n * 4 >= sms) return {2, 256};
+  return (long long)(div_up(rows, 128) + div_up(classes, 128)) * div_up(D, 128) * 2 >= sms ? Config{1, 128} : Config{1, 64};
 }
 int groups_of(const Config& c) { return c.bn >= 128 ? 2 : 1; }
 int clusters_of(const Config& c) { return device_sm_count() / c.cg; }
@@ -956,8 +972,9 @@ int launch_one(const Args& a, int items, cudaStream_t s) {
 template <int ROLE, typename E, int PIECES>
 int launch(const Config& c, const Args& a, int items, cudaStream_t s) {
   if (c.cg == 2) return launch_one<2, PIECES == 1 ? 256 : 128, ROLE, E, PIECES>(a, items, s);
-  if (c.bn == 128) return launch_one<1, 128, ROLE, E, PIECES>(a, items, s);
-  return launch_one<1, 64, ROLE, E, PIECES>(a, items, s);
+  if constexpr (!(ROLE == kGrad && PIECES == 3))
+    if (c.bn == 64) return launch_one<1, 64, ROLE, E, PIECES>(a, items, s);
+  return launch_one<1, 128, ROLE, E, PIECES>(a, items, s);
 }
 
 int pieces_of(int dtype) { return dtype == DK_F32 ? 3 : 1; }
@@ -974,7 +991,7 @@ struct ForwardPlan {
 ForwardPlan forward_plan(int T, int D, int V, int dtype) {
   ForwardPlan p;
   Layout l;
-  p.c = pick(T, V, pieces_of(dtype));
+  p.c = pick(T, V, D, pieces_of(dtype));
   p.tiles_m = div_up(T, 128 * p.c.cg), p.tiles_n = div_up(V, p.c.bn), p.slots = p.tiles_n * groups_of(p.c);
   p.few = few_rows(T, dtype);
   if (p.few) p.slots = few_slots(V);
@@ -1053,14 +1070,8 @@ BackwardPlan backward_plan(int T, int D, int V, int dtype) {
     const long long even = (long long)div_up(div_up(all, n), 256) * 256;
     side = even < all ? (int)even : all;
   }
-  p.dz = pick(p.tc, p.vc, pieces);
-  {
-    // the two products have tc x D and vc x D tiles
-    const int sms = device_sm_count(), wide_n = pieces == 1 ? 256 : 128;
-    const long long pairs = (long long)(div_up(p.tc, 256) + div_up(p.vc, 256)) * div_up(D, wide_n);
-    const long long wide = (long long)(div_up(p.tc, 128) + div_up(p.vc, 128)) * div_up(D, 128);
-    p.grad = pairs * 4 >= sms ? Config{2, wide_n} : wide * 2 >= sms ? Config{1, 128} : Config{1, 64};
-  }
+  p.dz = pick(p.tc, p.vc, D, pieces);
+  p.grad = pick_gradients(p.tc, p.vc, D, pieces);
   split_products(p, D, pieces);
   const bool lay = laid_out(D, dtype);
   const size_t row = (size_t)pitch_of(D) * 2 * pieces;

@@ -195,7 +195,8 @@ def test_head_sizes(t, d, v, dtype):
 
 
 # tiles shared by two SMs, in one or all products; several pieces of the classes, of the rows; long sums that are split
-LARGE = [(2100, 72, 5000), (1500, 520, 4600), (3000, 136, 24100), (24100, 40, 3001), (9000, 64, 40), (20, 72, 30000), (4700, 1032, 600)]
+LARGE = [(2100, 72, 5000), (1500, 520, 4600), (3000, 136, 24100), (24100, 40, 3001), (9000, 64, 40), (20, 72, 30000), (4700, 1032, 600), (1100, 1280, 1000),
+         (700, 256, 2100), (100, 264, 11000)]
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
