@@ -7,8 +7,8 @@
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011) with the seed as key
 // and (j / 8, offset) as counter gives the upper 16 bits of eight draws at once; their lower 16 bits come from the counter
 // with the highest bit of j / 8 set, and only a draw whose upper half equals the threshold's (one of 65536) looks at them.
-// With 32 bits of one word per element the generator, not memory, is the bound: 142 us against 102 for 154 M fp16 values
-// (308 MB in, 308 MB out, 6.0 TB/s; a copy kernel of the same shape without any generator takes 101).
+// With 32 bits of one word per element the generator, not memory, is the bound: 142 us against 106 for 154 M fp16 values
+// (308 MB in, 308 MB out, 5.8 TB/s; a copy of them takes 96).
 //
 // A dropped element is zero whatever x holds there (infinities and NaN included).  x / (1 - p) is a product with the fp32
 // (fp64) reciprocal, rounded once to the tensor's type.
@@ -149,8 +149,8 @@ template <> __device__ __forceinline__ __nv_bfloat16 times<__nv_bfloat16, float>
 }
 
 // Every element has its own draw; both tensors begin on 16 bytes, hold whole groups of eight (the elements of this launch), and the
-// threshold's upper half is below 0xffff.  A thread takes eight elements at a time, one counter's worth of draws.  All the warps an SM can hold, with registers to match, hide the
-// generator's latency: 102 us against 123 with the registers that ptxas takes by itself.
+// threshold's upper half is below 0xffff.  A thread takes eight elements at a time, one counter's worth of draws.  All the warps an SM can hold, with registers to
+// match, hide the generator's latency: 102 us against 123 with the registers that ptxas takes by itself.
 template <typename T, bool STATE>
 __global__ void __launch_bounds__(256, 8) dropout_kernel(const T* __restrict__ x, T* __restrict__ y, const DropArgs a) {
   constexpr int kPieces = 8 * sizeof(T) / 16;
