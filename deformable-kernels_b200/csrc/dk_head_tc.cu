@@ -833,52 +833,93 @@ template <typename T> __device__ __forceinline__ float as_float(T v) { return (f
 struct LayOut {
   const void* src;
   void* dst;
-  long long groups;          // of eight values of a row
-  int width, per_row;        // per_row: groups of a row
-  long long plane;           // values of a plane
+  long long rows;
+  int width, per_row;        // per_row: groups of eight values of a row
   const long long* target;   // rows whose target is `ignore` become zeros; NULL: all rows count
 };
-// [rows][width] -> PIECES planes [rows][8 per_row] of E: fp32 in three bf16 pieces, 16-bit rows on 16 bytes; eight values a thread
-template <typename T, typename E, int PIECES>
-__device__ __forceinline__ void lay_out_group(const LayOut& l, long long i, long long ignore) {
-  const long long r = l.groups < 0x7fffffff ? (long long)((unsigned)i / (unsigned)l.per_row) : i / l.per_row;
-  const int c = (int)(i - r * l.per_row) * 8;
-  const T* src = (const T*)l.src + r * l.width + c;
-  const bool in = !(l.target && l.target[r] == ignore);
-  T v[8];
-  if (in && l.width % 8 == 0) {
-    constexpr int kVec = 8 * sizeof(T) / 16;
+// `at`: the first of eight values of a row that begins anywhere, c: its column.  The aligned 16-byte pieces around them, moved into place; the last values of the
+// tensor, behind which there is no whole piece, go one by one.
+template <typename T>
+__device__ __forceinline__ void load_odd(T (&v)[8], const LayOut& l, long long at, int c) {
+  constexpr int kVec = 8 * sizeof(T) / 16;
+  const T* src = (const T*)l.src + at;
+  if (at + 8 + 16 / (int)sizeof(T) > l.rows * l.width) {
 #pragma unroll
-    for (int q = 0; q < kVec; ++q) reinterpret_cast<uint4*>(v)[q] = __ldg(reinterpret_cast<const uint4*>(src) + q);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = in && c + e < l.width ? src[e] : (T)0.0f;
+    for (int e = 0; e < 8; ++e) v[e] = c + e < l.width ? src[e] : (T)0.0f;
+    return;
   }
-  E out[PIECES][8];
+  const int off = (int)(reinterpret_cast<uintptr_t>(src) & 15);
+  const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(src) - off);
+  unsigned w[4 * (kVec + 1)];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if (PIECES == 1) {
-      out[0][e] = (E)v[e];
+  for (int q = 0; q <= kVec; ++q) {
+    const uint4 u = __ldg(from + q);
+    w[4 * q] = u.x, w[4 * q + 1] = u.y, w[4 * q + 2] = u.z, w[4 * q + 3] = u.w;
+  }
+#pragma unroll
+  for (int i = 0; i + 2 < 4 * (kVec + 1); ++i) w[i] = (off & 8) ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i + 1 < 4 * (kVec + 1); ++i) w[i] = (off & 4) ? w[i + 1] : w[i];
+  if (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4 * kVec; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < 4 * kVec; ++i) reinterpret_cast<unsigned*>(v)[i] = w[i];
+  if (c + 8 > l.width) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e >= l.width) v[e] = (T)0.0f;
+  }
+}
+// [rows][width] -> PIECES planes [rows][8 per_row] of E: fp32 in three bf16 pieces, 16-bit rows on 16 bytes; eight values a lane, `lanes` lanes a row
+template <typename T, typename E, int PIECES>
+__device__ __forceinline__ void lay_out_row(const LayOut& l, long long r, int first, int stride, long long ignore) {
+  const bool in = !(l.target && l.target[r] == ignore);
+  for (int g = first; g < l.per_row; g += stride) {
+    const long long at = r * l.width + g * 8;
+    alignas(16) T v[8];
+    if (!in) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (T)0.0f;
+    } else if (l.width % 8 == 0) {
+      constexpr int kVec = 8 * sizeof(T) / 16;
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) reinterpret_cast<uint4*>(v)[q] = __ldg(reinterpret_cast<const uint4*>((const T*)l.src + at) + q);
     } else {
-      float left = as_float(v[e]);
+      load_odd<T>(v, l, at, g * 8);
+    }
+    alignas(16) E out[PIECES][8];
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) {
-        out[p][e] = (E)left;
-        left -= as_float(out[p][e]);
+    for (int e = 0; e < 8; ++e) {
+      if (PIECES == 1) {
+        out[0][e] = (E)v[e];
+      } else {
+        float left = as_float(v[e]);
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+          out[p][e] = (E)left;
+          left -= as_float(out[p][e]);
+        }
       }
     }
-  }
+    const long long pitch = 8ll * l.per_row;
 #pragma unroll
-  for (int p = 0; p < PIECES; ++p) *reinterpret_cast<uint4*>((E*)l.dst + p * l.plane + i * 8) = *reinterpret_cast<const uint4*>(out[p]);
+    for (int p = 0; p < PIECES; ++p)
+      *reinterpret_cast<uint4*>((E*)l.dst + (p * l.rows + r) * pitch + 8 * g) = *reinterpret_cast<const uint4*>(out[p]);
+  }
 }
+// Rows of x, then of w; a warp has one at a time, or several short ones, or where there are few rows one of `parts` parts of one.
 template <typename T, typename E, int PIECES>
-__global__ void __launch_bounds__(256) lay_out_kernel(const LayOut x, const LayOut w, long long ignore) {
+__global__ void __launch_bounds__(256) lay_out_kernel(const LayOut x, const LayOut w, int lanes, int parts, long long ignore) {
   before_all();
   let_next();
-  const long long n = x.groups + w.groups;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    if (i < x.groups) lay_out_group<T, E, PIECES>(x, i, ignore);
-    else lay_out_group<T, E, PIECES>(w, i - x.groups, ignore);
+  const int lane = threadIdx.x & 31, at_once = 32 / lanes, part = blockIdx.x % parts, block = blockIdx.x / parts;
+  const int first = part * lanes + (lane & (lanes - 1)), stride = parts * lanes;
+  const long long n = x.rows + w.rows, step = (long long)(gridDim.x / parts) * 8 * at_once;
+  for (long long r = ((long long)block * 8 + (threadIdx.x >> 5)) * at_once + lane / lanes; r < n; r += step) {
+    if (r < x.rows) lay_out_row<T, E, PIECES>(x, r, first, stride, ignore);
+    else lay_out_row<T, E, PIECES>(w, r - x.rows, first, stride, ignore);
   }
 }
 
@@ -1108,10 +1149,16 @@ template <typename T, typename E, int PIECES>
 int operands(const void*& x, const void*& w, char* to_x, char* to_w, const long long* y, const Shape& h, int dtype, cudaStream_t s) {
   if (!laid_out(h.D, dtype)) return DK_OK;
   const int per_row = pitch_of(h.D) / 8;
-  LayOut lx = {x, to_x, (long long)h.T * per_row, h.D, per_row, (long long)h.T * per_row * 8, y};
-  LayOut lw = {w, to_w, (long long)h.V * per_row, h.D, per_row, (long long)h.V * per_row * 8, nullptr};
+  const LayOut lx = {x, to_x, h.T, h.D, per_row, y}, lw = {w, to_w, h.V, h.D, per_row, nullptr};
   x = to_x, w = to_w;
-  return launch_after(lay_out_kernel<T, E, PIECES>, blocks_for(lx.groups + lw.groups), 256, 0, 1, s, lx, lw, h.ignore);
+  int lanes = 1;
+  while (lanes < 32 && lanes < per_row) lanes *= 2;
+  // eight blocks an SM: as many parts of a row as it takes (1256 rows of 160 groups: 5 us in five parts, 8.6 in one)
+  const long long blocks = ((long long)h.T + h.V) * lanes / 256 + 1, most = (long long)device_sm_count() * 8;
+  int parts = 1;
+  while (blocks * (parts + 1) <= most && parts * lanes < per_row) ++parts;
+  return launch_after(lay_out_kernel<T, E, PIECES>, (unsigned)(blocks * parts < most ? blocks * parts : most / parts * parts), 256, 0, 1, s, lx,
+                      lw, lanes, parts, h.ignore);
 }
 template <typename E, int PIECES>
 bool operand_map(CUtensorMap* tm, const void* p, int rows, int width, int pitch, int box_rows = kBox) {
