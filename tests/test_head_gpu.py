@@ -430,6 +430,41 @@ def test_head_on_another_stream_and_captured():
             assert all(torch.equal(a, c) for a, c in zip(want, out))
 
 
+def test_one_row_without_a_batch_and_inference_mode():
+    f = functions()
+    x, w, y, b, _ = (t.to(DEV) for t in make(3, 40, 30, "fp32"))
+    each = f.linear_cross_entropy(x, w, y, b, reduction="none")
+    for reduction in ("none", "mean", "sum"):
+        one = f.linear_cross_entropy(x[1], w, y[1], b, reduction=reduction)
+        assert one.shape == () and abs(one - each[1]) < 1e-6
+    with torch.inference_mode():
+        assert torch.equal(f.linear_cross_entropy(x, w, y, b, reduction="none"), each)
+        assert torch.equal(f.dropout(x, 0.5, 3), f.dropout(x, 0.5, 3))
+
+
+def test_replays_whose_ignored_rows_become_strange():
+    """What an ignored row holds is looked at on the device: a captured step meets NaN in one replay and none in the next."""
+    f = functions()
+    x, w, y, b, up = make(300, 64, 500, "bf16", ignored=0.3, seed=40)
+    dead = y == -100
+    xs = x.to(DEV).requires_grad_(True)
+    ws = w.to(DEV).requires_grad_(True)
+    ys, bs = y.to(DEV), b.to(DEV)
+
+    def step():
+        loss = f.linear_cross_entropy(xs, ws, ys, bs)
+        return (loss.detach(),) + torch.autograd.grad(loss, [xs, ws])
+    want = [t.clone() for t in step()]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for bad in (0.0, float("nan"), 1.0, float("inf")):
+        with torch.no_grad():
+            xs[dead.to(DEV)] = bad
+        g.replay()
+        assert all(torch.equal(a, c) for a, c in zip(want, out)), bad
+
+
 def test_two_streams_at_once():
     """Calls of different sizes on two streams, none waiting for the other: each has its own scratch, and what is on the
     chip of an SM belongs to one block at a time."""
