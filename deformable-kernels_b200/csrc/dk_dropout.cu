@@ -28,6 +28,7 @@ struct DropArgs {
   double scale;
   unsigned long long first_group;  // of this launch: groups of eight elements, all with the same upper 32 bits
   unsigned groups;
+  int small;  // the index of a warp's part fits 32 bits
 };
 
 struct Key {
@@ -219,12 +220,57 @@ __global__ void __launch_bounds__(256) dropout_runs_kernel(const T* __restrict__
   }
 }
 
+// Long runs (planes, samples) of a multiple of eight elements, both tensors on 16 bytes: a warp has up to kPart elements of one run, so that the division and the
+// counter are its own and not those of every eight elements (28.9 M fp32 values in planes of 3136, p = 0.2: 35 us, 5.9 TB/s, against 41).
+constexpr int kPart = 1024;
+template <typename T, bool STATE>
+__global__ void __launch_bounds__(256) dropout_long_runs_kernel(const T* __restrict__ x, T* __restrict__ y, const DropArgs a, unsigned parts,
+                                                                unsigned long long units) {
+  constexpr int kEach = 16 / sizeof(T), kSteps = 4;  // values of a 16-byte piece; pieces in flight
+  using A = typename Compute<T>::type;
+  const Key key = key_of<STATE>(a);
+  const A scale = (A)a.scale;
+  const int lane = threadIdx.x & 31;
+  for (unsigned long long u = (unsigned long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (unsigned long long)gridDim.x * 8) {
+    const unsigned long long j = a.small ? (unsigned long long)((unsigned)u / parts) : u / parts;
+    const unsigned long long in_run = (u - j * parts) * kPart, left = a.run - in_run;
+    const int n = left < kPart ? (int)left : kPart;
+    const T* from = x + j * a.run + in_run;
+    T* to = y + j * a.run + in_run;
+    const bool keep = kept8(j >> 3, key, a.hi, a.lo) >> (j & 7) & 1;
+    const bool all[8] = {keep, keep, keep, keep, keep, keep, keep, keep};
+    for (int e0 = lane * kEach; e0 < n; e0 += 32 * kEach * kSteps) {
+      uint4 v[kSteps];
+#pragma unroll
+      for (int q = 0; q < kSteps; ++q) {
+        const int e = e0 + q * 32 * kEach;
+        v[q] = keep && e < n ? __ldg(reinterpret_cast<const uint4*>(from + e)) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int q = 0; q < kSteps; ++q) {
+        const int e = e0 + q * 32 * kEach;
+        Piece<T>::apply(v[q], scale, all);
+        if (e < n) *reinterpret_cast<uint4*>(to + e) = v[q];
+      }
+    }
+  }
+}
+
 template <typename T, bool STATE>
 int launch_dropout(const void* input, void* output, DropArgs a, cudaStream_t s) {
   const T* x = (const T*)input;
   T* y = (T*)output;
   const bool vector = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0;
   const unsigned most = (unsigned)device_sm_count() * 32;
+  if (vector && a.run >= 256 && a.run % 8 == 0) {
+    const unsigned long long parts = (a.run + kPart - 1) / kPart, units = a.count / a.run * parts;
+    if (a.count % a.run == 0 && parts <= 0xffffffffull) {
+      a.small = units <= 0xffffffffull;
+      const unsigned long long blocks = (units + 7) / 8;
+      dropout_long_runs_kernel<T, STATE><<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(x, y, a, (unsigned)parts, units);
+      return check_launch();
+    }
+  }
   unsigned long long at = 0, total = (a.count + 7) >> 3;
   while (at < total) {
     unsigned long long n = total - at < 1ull << 30 ? total - at : 1ull << 30;

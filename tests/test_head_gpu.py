@@ -25,7 +25,7 @@ def no_wait_ran_out():
 
 @pytest.mark.parametrize("dtype", list(H.DTYPES))
 @pytest.mark.parametrize("shape, shared", [((1,), 0), ((7,), 0), ((8,), 0), ((9, 3), 1), ((300, 1001), 0), ((5, 6, 7, 9), 2), ((5, 6, 7, 9), 3),
-                                           ((4, 3, 64, 64), 2), ((3, 5, 2), 1), ((2, 3), 2), ((), 0)])
+                                           ((4, 3, 64, 64), 2), ((3, 7, 8, 32), 2), ((2, 5, 41, 40), 2), ((6, 3, 40, 40), 3), ((3, 5, 2), 1), ((2, 3), 2), ((), 0)])
 def test_dropout_is_its_definition(shape, shared, dtype):
     torch.manual_seed(1)
     x = torch.randn(shape).to(H.DTYPES[dtype])
