@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
             __syncwarp();
             if (lane == 0) store_box(&a.dz_out, stage, col_base + c0, row_base, pc);
             if (a.column_sums) {
-              // two columns a lane
+              // two columns a lane, of dz as the products see it: rounded, with 32-bit sums
 #pragma unroll 8
               for (int r = 0; r < 32; ++r) {
                 const float2 f = unpack<E>(lds4(staged(stage, r, lane >> 2) + (lane & 3) * 4));

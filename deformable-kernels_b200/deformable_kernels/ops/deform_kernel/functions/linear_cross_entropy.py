@@ -8,6 +8,9 @@ as ``torch.nn.functional.cross_entropy(linear(input, weight, bias), target, ...)
 time; neither they nor their gradient ever exist as a whole.  The loss is float32 (float64 for float64 inputs).  Weights and biases
 that differ in dtype from the features follow them.
 
+Logits, sums and statistics are fp32 for 16-bit and fp32 inputs (fp64 for fp64); for 16-bit inputs the gradient of the logits is rounded
+to 16 bits between the products, as it would be as a tensor of its own.  The same call gives the same bits.
+
 Rows whose target is ``ignore_index`` have no loss and no gradient whatever their features hold.  A target that is no class makes the loss
 NaN.  Features or weights that are not finite make the losses of the rows they reach NaN; a bias of -inf takes a class out.
 """
