@@ -86,7 +86,7 @@ int launch_combine(const Partials<A>& p, const long long* y, int slots, void* lo
                    cudaStream_t s);
 inline unsigned* combine_count(double* partial, int T) { return (unsigned*)(partial + 3ll * div_up(T, kCombineRows)); }
 
-// ---- the loss of a few rows (dk_head.cu): memory is the bound, the products are taken on the CUDA cores
+// ---- the loss of a few rows without a backward (dk_head.cu): memory is the bound, the products are taken on the CUDA cores
 bool few_rows(int T, int dtype);
 int few_slots(int V);
 template <typename T>

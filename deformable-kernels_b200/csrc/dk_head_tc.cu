@@ -1029,12 +1029,13 @@ struct ForwardPlan {
   bool few;
   size_t x, w, top, sum, all, picked, partial, bytes;
 };
-ForwardPlan forward_plan(int T, int D, int V, int dtype) {
+// few: the CUDA cores' form, for a few rows without a backward
+ForwardPlan forward_plan(int T, int D, int V, int dtype, bool few) {
   ForwardPlan p;
   Layout l;
   p.c = pick(T, V, D, pieces_of(dtype));
   p.tiles_m = div_up(T, 128 * p.c.cg), p.tiles_n = div_up(V, p.c.bn), p.slots = p.tiles_n * groups_of(p.c);
-  p.few = few_rows(T, dtype);
+  p.few = few;
   if (p.few) p.slots = few_slots(V);
   const bool lay = !p.few && laid_out(D, dtype);
   const size_t row = (size_t)pitch_of(D) * 2 * pieces_of(dtype);
@@ -1169,8 +1170,9 @@ bool operand_map(CUtensorMap* tm, const void* p, int rows, int width, int pitch,
 template <typename T, typename E, int PIECES>
 int forward(const void* x, const void* w, const void* b, const long long* y, void* loss, void* saved, const Shape& h, int dtype, void* ws,
             size_t ws_bytes, cudaStream_t s) {
-  const ForwardPlan p = forward_plan(h.T, h.D, h.V, dtype);
-  if (!ws || ws_bytes < p.bytes) return DK_ERR_WORKSPACE;
+  // With a backward to come the logits have to be the ones that it will compute: where p is nearly one, p - 1 is the difference of the two.
+  const ForwardPlan p = forward_plan(h.T, h.D, h.V, dtype, few_rows(h.T, dtype) && !saved);
+  if (!ws || ws_bytes < tc_forward_bytes(h.T, h.D, h.V, dtype)) return DK_ERR_WORKSPACE;
   char* m = (char*)ws;
   if (p.few) {
     const Partials<float> part = {(float*)(m + p.top), (float*)(m + p.sum), (float*)(m + p.all), (float*)(m + p.picked)};
@@ -1283,7 +1285,10 @@ int backward(const void* up, const void* x, const void* w, const void* b, const 
 
 }  // namespace
 
-size_t tc_forward_bytes(int T, int D, int V, int dtype) { return forward_plan(T, D, V, dtype).bytes; }
+size_t tc_forward_bytes(int T, int D, int V, int dtype) {
+  const size_t n = forward_plan(T, D, V, dtype, false).bytes, few = few_rows(T, dtype) ? forward_plan(T, D, V, dtype, true).bytes : 0;
+  return n > few ? n : few;
+}
 size_t tc_backward_bytes(int T, int D, int V, int dtype) { return backward_plan(T, D, V, dtype).bytes; }
 
 int tc_forward(const void* x, const void* w, const void* b, const long long* y, void* loss, void* saved, const Shape& h, int dtype,

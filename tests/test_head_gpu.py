@@ -180,7 +180,11 @@ def check(x, w, y, b, up, where="", device="cpu", **kw):
         assert over <= 1, (where, name, over, (v.double() - out[name]).abs().max().item(), out[name].abs().max().item())
     with torch.no_grad():
         again = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), leaves[2] if b is not None else None, **kw)
-    assert torch.equal(again, loss.detach()) or not torch.isfinite(again).all()
+    if x.shape[0] > 8:  # a few rows without a backward are summed in another order
+        assert torch.equal(again, loss.detach()) or not torch.isfinite(again).all()
+    else:
+        over = ((again.cpu().double() - out["loss"]).abs() / far["loss"]).nan_to_num(0).max().item()
+        assert over <= 1 and again.shape == loss.shape and torch.isfinite(again).all() == torch.isfinite(out["loss"]).all(), (where, over)
     return got
 
 
@@ -302,6 +306,34 @@ def test_losses_near_zero(rows, dtype):
         got = functions().linear_cross_entropy(x.to(dt).to(DEV), w.to(dt).to(DEV), y.to(DEV)).item()
         want = torch.log1p(torch.exp(torch.tensor(-gap, dtype=torch.double))).item()
         assert abs(got - want) < 2.0 ** -23 + 2.0 ** -21 * want
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 40])
+def test_gradients_of_losses_near_zero(rows):
+    """p - 1 of a class that is nearly certain: it takes the backward's logits to be the forward's.  fp32 features whose
+    products are not exact; dz is off by the logits' error relative to itself (1e-5 at these sizes, 64 products of a
+    few units) and by three roundings of one, 2^-22, against 1 - p."""
+    gen = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, 64, generator=gen)
+    y = torch.arange(rows) % 4
+    for lift in (9.0, 11.0):
+        w = torch.randn(5, 64, generator=gen) * 0.05
+        x2 = x.clone()
+        b = torch.zeros(5)
+        # the row's own class lifted through its features: x . w_y = lift, about nothing for the others
+        for t in range(rows):
+            x2[t] = x[t] * 0.1 + lift * w[y[t]] / w[y[t]].square().sum()
+        leaves = [t.to(DEV).requires_grad_(True) for t in (x2, w, b)]
+        loss = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), leaves[2])
+        got = torch.autograd.grad(loss, leaves)
+        ref = [t.double().requires_grad_(True) for t in (x2, w, b)]
+        z = ref[0] @ ref[1].t() + ref[2]
+        want = torch.autograd.grad(torch.nn.functional.cross_entropy(z, y), ref)
+        rest = 1 - torch.softmax(z.detach(), 1).gather(1, y[:, None]).min().item()
+        least = 1 - torch.softmax(z.detach(), 1).gather(1, y[:, None]).max().item()
+        assert rest < 0.1
+        for a, c in zip(got, want):
+            assert (a.cpu().double() - c).norm() < (1e-5 + 2.0 ** -22 / least) * c.norm()
 
 
 def test_leading_dimensions_views_and_dtypes():
