@@ -771,6 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           if (row_base >= p.M || col_base + c0 >= p.N) break;  // of the whole warp
           float v[32];
           columns(v, c0);
+          __syncwarp();  // the lanes have read what the 32 columns before left in the staging buffer
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             sts16(staged(stage, lane, q), __float_as_uint(v[4 * q] * back), __float_as_uint(v[4 * q + 1] * back),

@@ -1,0 +1,37 @@
+"""The classifier head on the GPU where its kernels end: ragged tiles, long sums, values at the ends of a type's range, layouts,
+second derivatives, waits that run out."""
+import pytest
+import torch
+
+import head_oracle as H
+from test_head_gpu import DEV, check, functions, make, no_wait_ran_out  # noqa: F401  (the fixture watches every test)
+
+pytestmark = pytest.mark.gpu
+
+
+def padded(x, w, y, b, rows, classes):
+    """The same call with `rows` more rows, which are ignored, and `classes` more classes, which a bias of -inf takes out."""
+    t, d = x.shape
+    x2 = torch.cat([x, torch.randn(rows, d, generator=torch.Generator().manual_seed(1)).to(x.dtype)])
+    w2 = torch.cat([w, torch.randn(classes, d, generator=torch.Generator().manual_seed(2)).to(w.dtype)])
+    return x2, w2, torch.cat([y, torch.full((rows,), -100)]), torch.cat([b, torch.full((classes,), float("-inf"), dtype=b.dtype)])
+
+
+@pytest.mark.parametrize("features", [33, 72, 200])
+@pytest.mark.parametrize("rows, classes", [(r, c) for r in (1, 2, 3, 5, 31, 33, 62, 63) for c in (7, 30, 63)] + [(1501, 130), (130, 9001)])
+def test_fp32_gradients_of_ragged_tiles_are_those_of_whole_ones(rows, classes, features):
+    """The last tile of rows and of classes ends anywhere: nothing that its lanes skip changes what the others store.  The same
+    call with whole tiles adds zeros only (ignored rows, classes without a chance): the same bits, call after call.  Short sums,
+    and long ones that are split and joined."""
+    x, w, y, b, _ = make(rows, features, classes, "fp32", seed=rows + classes)
+    more = -rows % 64, -classes % 64
+
+    def grads(x, w, y, b):
+        leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+        loss = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), leaves[2], reduction="sum")
+        return torch.autograd.grad(loss, leaves)
+    want = [t[:n] for t, n in zip(grads(*padded(x, w, y, b, *more)), (rows, classes, classes))]
+    for _ in range(3):
+        got = grads(x, w, y, b)
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+    check(x, w, y, b, torch.tensor(1.0), reduction="sum")
