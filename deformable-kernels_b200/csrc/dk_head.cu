@@ -11,6 +11,7 @@
 // logits of the piece once more, dz of the piece into the workspace, then the two products.
 //
 // Here: the C entry points, the kernel that joins a row's tiles, and fp64 on the CUDA cores.  The other types: dk_head_tc.cu.
+#include <limits.h>
 #include <math_constants.h>
 
 #include "dk_head.cuh"
@@ -501,6 +502,12 @@ int backward64(const void* up, const double* x, const double* w, const double* b
 }
 
 bool shape_ok(int rows, int features, int classes) { return rows > 0 && features > 0 && classes > 0; }
+// Loops and tiles step past a size by up to 19 thousand (few_rows_kernel: 4 blocks an SM, 32 classes a block); their indices are 32-bit.
+// The bytes of dz as a whole, from which its pieces are planned, are a 64-bit number.
+constexpr int kLargest = INT_MAX - 0xffff;
+bool sizes_fit(int rows, int features, int classes) {
+  return rows <= kLargest && features <= kLargest && classes <= kLargest && (long long)rows * classes <= 1ll << 56;
+}
 bool dtype_ok(int d) { return d == DK_F32 || d == DK_F16 || d == DK_BF16 || d == DK_F64; }
 bool options_ok(int reduction, double smoothing) {
   return reduction >= DK_REDUCE_NONE && reduction <= DK_REDUCE_SUM && smoothing >= 0.0 && smoothing <= 1.0;
@@ -517,7 +524,7 @@ using namespace dk;
 extern "C" {
 
 size_t dk_linear_cross_entropy_forward_workspace_bytes(int rows, int features, int classes, int dtype) {
-  if (!head::shape_ok(rows, features, classes) || !head::dtype_ok(dtype)) return 0;
+  if (!head::shape_ok(rows, features, classes) || !head::dtype_ok(dtype) || !head::sizes_fit(rows, features, classes)) return 0;
   return dtype == DK_F64 ? head::forward_plan(rows, classes).bytes : head::tc_forward_bytes(rows, features, classes, dtype);
 }
 
@@ -527,6 +534,7 @@ int dk_linear_cross_entropy_forward(const void* input, const void* weight, const
   if (!input || !weight || !target || !loss || !head::shape_ok(rows, features, classes) || !head::dtype_ok(dtype) ||
       !head::options_ok(reduction, label_smoothing) || !head::aligned16(input, weight) || !head::aligned16(workspace, nullptr))
     return DK_ERR_BAD_ARGUMENT;
+  if (!head::sizes_fit(rows, features, classes)) return DK_ERR_UNSUPPORTED;
   const head::Shape h = {rows, features, classes, ignore_index, reduction, label_smoothing};
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == DK_F64)
@@ -536,7 +544,7 @@ int dk_linear_cross_entropy_forward(const void* input, const void* weight, const
 }
 
 size_t dk_linear_cross_entropy_backward_workspace_bytes(int rows, int features, int classes, int dtype) {
-  if (!head::shape_ok(rows, features, classes) || !head::dtype_ok(dtype)) return 0;
+  if (!head::shape_ok(rows, features, classes) || !head::dtype_ok(dtype) || !head::sizes_fit(rows, features, classes)) return 0;
   return dtype == DK_F64 ? head::backward_plan(rows, classes).bytes : head::tc_backward_bytes(rows, features, classes, dtype);
 }
 
@@ -548,6 +556,7 @@ int dk_linear_cross_entropy_backward(const void* grad_loss, const void* input, c
       !head::options_ok(reduction, label_smoothing) || !head::aligned16(input, weight) || !head::aligned16(grad_input, grad_weight) ||
       !head::aligned16(workspace, nullptr))
     return DK_ERR_BAD_ARGUMENT;
+  if (!head::sizes_fit(rows, features, classes)) return DK_ERR_UNSUPPORTED;
   if (!grad_input && !grad_weight && !grad_bias) return DK_OK;
   const head::Shape h = {rows, features, classes, ignore_index, reduction, label_smoothing};
   cudaStream_t s = (cudaStream_t)stream;

@@ -304,7 +304,8 @@ int dk_dropout(const void *input, void *output, long long count, long long run, 
  * loss is NaN, the gradients are zero).  loss: one value, or [rows] for DK_REDUCE_NONE; it, `saved` and grad_loss are
  * float (double for DK_F64).  saved: 2 rows + 2 values that the backward takes back, or
  * NULL.  input, weight,
- * their gradients and the workspace begin on 16 bytes.  Any gradient may be NULL. */
+ * their gradients and the workspace begin on 16 bytes.  Any gradient may be NULL.
+ * DK_ERR_UNSUPPORTED: a size above 2^31 - 65536, more than 2^56 logits. */
 typedef enum dk_reduction { DK_REDUCE_NONE = 0, DK_REDUCE_MEAN = 1, DK_REDUCE_SUM = 2 } dk_reduction;
 size_t dk_linear_cross_entropy_forward_workspace_bytes(int rows, int features, int classes, int dtype);
 int dk_linear_cross_entropy_forward(const void *input, const void *weight, const void *bias, const long long *target,

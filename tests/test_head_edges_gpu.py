@@ -35,3 +35,15 @@ def test_fp32_gradients_of_ragged_tiles_are_those_of_whole_ones(rows, classes, f
         got = grads(x, w, y, b)
         assert all(torch.equal(a, c) for a, c in zip(got, want))
     check(x, w, y, b, torch.tensor(1.0), reduction="sum")
+
+
+def test_more_classes_than_the_kernels_count_are_refused():
+    from deformable_kernels._cabi import DkError
+    w = torch.zeros(2 ** 31 - 1, 1, dtype=torch.float16, device=DEV)
+    x, y = torch.zeros(1, 1, dtype=torch.float16, device=DEV), torch.zeros(1, dtype=torch.int64, device=DEV)
+    with pytest.raises(DkError, match="unsupported|supported"):
+        functions().linear_cross_entropy(x, w, y)
+    with pytest.raises(DkError):
+        functions().linear_cross_entropy(x.requires_grad_(True), w, y)
+    del w
+    torch.cuda.empty_cache()
