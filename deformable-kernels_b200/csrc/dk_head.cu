@@ -523,6 +523,8 @@ using namespace dk;
 
 extern "C" {
 
+long long dk_linear_cross_entropy_wait_limit(long long nanoseconds) { return head::set_wait_limit(nanoseconds); }
+
 size_t dk_linear_cross_entropy_forward_workspace_bytes(int rows, int features, int classes, int dtype) {
   if (!head::shape_ok(rows, features, classes) || !head::dtype_ok(dtype) || !head::sizes_fit(rows, features, classes)) return 0;
   return dtype == DK_F64 ? head::forward_plan(rows, classes).bytes : head::tc_forward_bytes(rows, features, classes, dtype);

@@ -113,6 +113,7 @@ int launch_after(K kernel, unsigned grid, unsigned block, size_t smem, int clust
 size_t tc_forward_bytes(int T, int D, int V, int dtype);
 int tc_forward(const void* x, const void* w, const void* b, const long long* y, void* loss, void* saved, const Shape& h, int dtype,
                void* ws, size_t ws_bytes, cudaStream_t s);
+long long set_wait_limit(long long nanoseconds);  // of the launches from now on; the one before
 size_t tc_backward_bytes(int T, int D, int V, int dtype);
 int tc_backward(const void* up, const void* x, const void* w, const void* b, const long long* y, const void* saved, void* dx, void* dw,
                 void* db, const Shape& h, int dtype, void* ws, size_t ws_bytes, cudaStream_t s);

@@ -21,6 +21,7 @@
 
 #include <math_constants.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "dk_head.cuh"
@@ -34,6 +35,8 @@ using ring::smem_u32;
 namespace {
 
 __device__ int g_head_error;  // set when a bounded wait ran out
+constexpr unsigned long long kWaitLimit = 2000000000;  // nanoseconds
+std::atomic<unsigned long long> g_wait_limit{kWaitLimit};
 
 constexpr int kBox = 64;                    // values per side of a TMA box
 constexpr int kBoxBytes = kBox * kBox * 2;  // 8192
@@ -196,19 +199,26 @@ __device__ __forceinline__ unsigned long long nanoseconds() {
   asm volatile("mov.u64 %0, %%globaltimer;\n" : "=l"(t));
   return t;
 }
-// Two seconds: the longest sum a tile can have (2^27 values of dz in one piece, 65536 steps for a tile 32 wide) takes some 20 ms.
-__device__ __forceinline__ bool wait(unsigned bar, unsigned parity, volatile int* abort_flag) {
-  bool done = try_wait(bar, parity);
-  if (!done) {
-    const unsigned long long start = nanoseconds();
-    for (unsigned i = 1; !done && !*abort_flag; ++i) {
-      done = try_wait(bar, parity);
-      if ((i & 63) == 0 && nanoseconds() - start > 2000000000ull) break;
-      if (i == 1u << 30) break;
+// True once any thread of the block gave up: `limit` nanoseconds without the phase.  Of the time between two polls ten milliseconds count at
+// most: a process that is suspended for longer has not waited.
+constexpr unsigned long long kMostBetweenPolls = 10000000;
+__device__ __forceinline__ bool wait(unsigned bar, unsigned parity, volatile int* abort_flag, unsigned long long limit) {
+  bool gone = *abort_flag != 0;
+  if (!gone && !try_wait(bar, parity)) {
+    unsigned long long last = nanoseconds(), spent = 0;
+    gone = true;
+    for (unsigned i = 0; i < 1u << 30; ++i) {
+      if (try_wait(bar, parity)) {
+        gone = false;
+        break;
+      }
+      const unsigned long long now = nanoseconds(), step = now - last;
+      spent += step < kMostBetweenPolls ? step : kMostBetweenPolls, last = now;
+      if (*abort_flag || spent > limit) break;
     }
+    if (gone) *abort_flag = 1;
   }
-  if (!done) *abort_flag = 1;
-  return __any_sync(0xffffffffu, *abort_flag != 0);
+  return __any_sync(0xffffffffu, gone);
 }
 
 // 16-byte piece q of row r in a staging buffer of 128-byte rows
@@ -287,6 +297,7 @@ struct Args {
   int width;                  // of x
   int up_rows;                // of the call
   const long long* target_all;
+  unsigned long long wait_limit;  // nanoseconds
   // gradients
   Product dw, dx;
   Schedule schedule;
@@ -449,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
       for (int kb = it.first; kb < it.first + it.count; ++kb) {
         for (int piece = 0; piece < PIECES; ++piece, ++fill) {
           const int s = fill % kStages;
-          if (wait(smem_u32(&t.empty[s]), ((fill / kStages) & 1) ^ 1, abort_flag)) continue;
+          if (wait(smem_u32(&t.empty[s]), ((fill / kStages) & 1) ^ 1, abort_flag, a.wait_limit)) continue;
           const unsigned sa = base + s * kStage, sb = sa + 128 * 128;
           unsigned bar = smem_u32(&t.full[s]);
           if (CG == 2) bar = map_rank(bar, 0);
@@ -474,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
     // every stage handed back: nothing of this block is in flight any more
     for (int s = 0; s < kStages && s < fill; ++s) {
       const int last = (fill - 1 - s) / kStages * kStages + s;
-      (void)wait(smem_u32(&t.empty[s]), (last / kStages) & 1, abort_flag);
+      (void)wait(smem_u32(&t.empty[s]), (last / kStages) & 1, abort_flag, a.wait_limit);
     }
   } else if (warp == 1) {
     // ---------------- mma, the leading block only
@@ -491,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         const unsigned lead = kBoxBytes, step_a = ta ? 2048 : 32, step_b = tb ? 2048 : 32;
         for (int k0 = 0; k0 < it.count; k0 += kChunk, ++round) {
           const int b = round & 1, end = it.count - k0 < kChunk ? it.count : k0 + kChunk;
-          bool gone = wait(smem_u32(&t.acc_empty[b]), ((round >> 1) & 1) ^ 1, abort_flag);
+          bool gone = wait(smem_u32(&t.acc_empty[b]), ((round >> 1) & 1) ^ 1, abort_flag, a.wait_limit);
           tc::fence_after();
           const unsigned d = tmem + b * kAcc;
           for (int k = k0; k < end; ++k, fill += PIECES) {
@@ -499,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
 #pragma unroll
             for (int p = 0; p < PIECES; ++p) {
               const int s = (fill + p) % kStages;
-              gone = wait(smem_u32(&t.full[s]), ((fill + p) / kStages) & 1, abort_flag);
+              gone = wait(smem_u32(&t.full[s]), ((fill + p) / kStages) & 1, abort_flag, a.wait_limit);
               if (gone) break;
               tc::fence_after();
               const unsigned sa = base + s * kStage;
@@ -595,21 +606,22 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
       if (more) ask(ahead, next);
       const long long y = row < a.rows ? now.y : -1;
       const bool live = ROLE == kDz && row < a.rows && y != a.ignore;
-      const float ref = now.ref, inv = now.inv, g = y >= 0 && y < a.all_classes ? now.up * unit : CUDART_NAN_F;  // of a live row
+      const float ref = now.ref, inv = now.inv;
       // the row's own class as a column of this warp, -1: elsewhere
       const long long far = y - a.class0 - col_base;
       const int own = far >= 0 && far < kWide ? (int)far : -1;
       const int b = round & 1;
       const unsigned d = tmem + lanes + b * kAcc + grp * kWide;
       float got[PIECES == 1 ? 1 : 2][32];  // fp32: the sums
+      bool gone = false;  // the products never came: what the tile leaves is NaN
       if (PIECES == 1) {
-        (void)wait(smem_u32(&t.acc_full[b]), (round >> 1) & 1, abort_flag);
+        gone = wait(smem_u32(&t.acc_full[b]), (round >> 1) & 1, abort_flag, a.wait_limit);
         tc::fence_after();
         ++round;
       } else {
         for (int k = 0; k < it.count; k += kChunk, ++round) {
           const int bk = round & 1;
-          (void)wait(smem_u32(&t.acc_full[bk]), (round >> 1) & 1, abort_flag);
+          gone |= wait(smem_u32(&t.acc_full[bk]), (round >> 1) & 1, abort_flag, a.wait_limit);
           tc::fence_after();
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
@@ -619,6 +631,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           release(bk);
         }
       }
+      const float g = !gone && y >= 0 && y < a.all_classes ? now.up * unit : CUDART_NAN_F;  // of a live row
+      const float factor = gone ? CUDART_NAN_F : back;
       // 32 columns from c on
       auto columns = [&](float (&v)[32], int c) {
         if (PIECES == 1) {
@@ -667,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
         }
         if (row < a.rows) {
           const long long at = (long long)(it.n * kGroups + grp) * a.rows + row;
-          a.top[at] = top, a.sum[at] = sum;
+          a.top[at] = top, a.sum[at] = gone ? CUDART_NAN_F : sum;
           if (a.all) a.all[at] = all;
           if (own >= 0 && own + col_base < a.classes) a.picked[row] = picked;
         }
@@ -753,8 +767,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
               const float* f = &v[q >> 2][(q & 3) * 8];
-              sts16(staged(stage, lane, q), pack<E>(f[0] * back, f[1] * back), pack<E>(f[2] * back, f[3] * back),
-                    pack<E>(f[4] * back, f[5] * back), pack<E>(f[6] * back, f[7] * back));
+              sts16(staged(stage, lane, q), pack<E>(f[0] * factor, f[1] * factor), pack<E>(f[2] * factor, f[3] * factor),
+                    pack<E>(f[4] * factor, f[5] * factor), pack<E>(f[6] * factor, f[7] * factor));
             }
             __syncwarp();
             const int c = col_base + c0 + 8 * (lane & 7);
@@ -774,8 +788,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           __syncwarp();  // the lanes have read what the 32 columns before left in the staging buffer
 #pragma unroll
           for (int q = 0; q < 8; ++q)
-            sts16(staged(stage, lane, q), __float_as_uint(v[4 * q] * back), __float_as_uint(v[4 * q + 1] * back),
-                  __float_as_uint(v[4 * q + 2] * back), __float_as_uint(v[4 * q + 3] * back));
+            sts16(staged(stage, lane, q), __float_as_uint(v[4 * q] * factor), __float_as_uint(v[4 * q + 1] * factor),
+                  __float_as_uint(v[4 * q + 2] * factor), __float_as_uint(v[4 * q + 3] * factor));
           __syncwarp();
           if (vec) {
             // eight lanes a row: four values each
@@ -1189,6 +1203,7 @@ int forward(const void* x, const void* w, const void* b, const long long* y, voi
   a.rows = h.T, a.classes = h.V, a.depth = div_up(h.D, kBox);
   a.tiles_m = p.tiles_m, a.tiles_n = p.tiles_n, a.group = row_group(p.c, h.D, PIECES, p.tiles_m);
   a.bias = b, a.target = y, a.ignore = h.ignore;
+  a.wait_limit = g_wait_limit.load(std::memory_order_relaxed);
   a.top = (float*)(m + p.top), a.sum = (float*)(m + p.sum), a.all = h.smoothing != 0.0 ? (float*)(m + p.all) : nullptr;
   a.picked = (float*)(m + p.picked), a.done = combine_count((double*)(m + p.partial), h.T);
   if ((long long)p.tiles_m * p.tiles_n > 0x3fffffff) return DK_ERR_UNSUPPORTED;
@@ -1221,6 +1236,7 @@ int backward(const void* up, const void* x, const void* w, const void* b, const 
       !operand_map<E, PIECES>(&a.x_clean, m + p.x, h.T, h.D, pitch))
     return DK_ERR_CUDA;
   a.depth = div_up(h.D, kBox), a.bias = b, a.ignore = h.ignore, a.all_classes = h.V;
+  a.wait_limit = g_wait_limit.load(std::memory_order_relaxed);
   a.up = {(const float*)up, stat + 2ll * h.T, largest, h.reduction, 1.0f};
   // up to one half: beyond, p unit would leave fp16's range
   if (h.reduction != DK_REDUCE_NONE)
@@ -1308,6 +1324,10 @@ int tc_backward(const void* up, const void* x, const void* w, const void* b, con
     case DK_BF16: return backward<__nv_bfloat16, __nv_bfloat16, 1>(up, x, w, b, y, saved, dx, dw, db, h, dtype, ws, ws_bytes, s);
     default: return backward<float, __nv_bfloat16, 3>(up, x, w, b, y, saved, dx, dw, db, h, dtype, ws, ws_bytes, s);
   }
+}
+
+long long set_wait_limit(long long nanoseconds) {
+  return (long long)g_wait_limit.exchange(nanoseconds > 0 ? (unsigned long long)nanoseconds : kWaitLimit);
 }
 
 // Code of the last bounded wait that ran out on the current device (0 = none); synchronises with the device.

@@ -71,6 +71,7 @@ _PROTOS = {
     "dk_offset_clip_backward": (_int, [_vp, _vp, _vp, _vp, _int, _int, _int] + [ctypes.c_double] * 4 + [_int, _vp]),
     "dk_dropout": (_int, [_vp, _vp, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_double, ctypes.c_ulonglong,
                           ctypes.c_ulonglong, _vp, _vp, _int, _vp]),
+    "dk_linear_cross_entropy_wait_limit": (ctypes.c_longlong, [ctypes.c_longlong]),
     "dk_linear_cross_entropy_forward_workspace_bytes": (_sz, [_int] * 4),
     "dk_linear_cross_entropy_forward": (_int, [_vp] * 6 + [_int] * 3 + [ctypes.c_longlong, _int, ctypes.c_double, _int, _vp, _sz, _vp]),
     "dk_linear_cross_entropy_backward_workspace_bytes": (_sz, [_int] * 4),

@@ -306,6 +306,11 @@ int dk_dropout(const void *input, void *output, long long count, long long run, 
  * NULL.  input, weight,
  * their gradients and the workspace begin on 16 bytes.  Any gradient may be NULL.
  * DK_ERR_UNSUPPORTED: a size above 2^31 - 65536, more than 2^56 logits. */
+/* The kernels wait for their own copies and products only, and no wait goes on for ever: after two seconds (time for which the
+ * process is suspended does not count) the kernel ends, what it could not compute is NaN (losses, gradients), and
+ * dk_ring_error_status() says so.  dk_linear_cross_entropy_wait_limit sets that limit, in nanoseconds, for the calls
+ * of this process from now on (0: two seconds) and returns the one before. */
+long long dk_linear_cross_entropy_wait_limit(long long nanoseconds);
 typedef enum dk_reduction { DK_REDUCE_NONE = 0, DK_REDUCE_MEAN = 1, DK_REDUCE_SUM = 2 } dk_reduction;
 size_t dk_linear_cross_entropy_forward_workspace_bytes(int rows, int features, int classes, int dtype);
 int dk_linear_cross_entropy_forward(const void *input, const void *weight, const void *bias, const long long *target,

@@ -47,3 +47,58 @@ def test_more_classes_than_the_kernels_count_are_refused():
         functions().linear_cross_entropy(x.requires_grad_(True), w, y)
     del w
     torch.cuda.empty_cache()
+
+
+WAITS = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch
+from deformable_kernels import _cabi as C
+import test_head_gpu as T
+ran_out = 0
+for rows, features, classes, dtype, kw in %r:
+    x, w, y, b, up = T.make(rows, features, classes, dtype, ignored=0.1, reduction="none")
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    y, up = y.cuda(), up.cuda()
+
+    def step():
+        loss = T.functions().linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], reduction="none", **kw)
+        return [loss.detach()] + list(torch.autograd.grad(loss, leaves, up))
+    assert C.lib.dk_linear_cross_entropy_wait_limit(0) in (1, 2000000000)
+    want = step()
+    torch.cuda.synchronize()
+    before = C.lib.dk_ring_error_status()
+    assert C.lib.dk_linear_cross_entropy_wait_limit(1) == 2000000000
+    got = step()
+    torch.cuda.synchronize()
+    after = C.lib.dk_ring_error_status()
+    gave_up = [bool(torch.isnan(a).any()) for a in got]
+    for a, c in zip(got, want):
+        assert not torch.isnan(c).any()
+        assert (torch.isnan(a) | (a == c)).all(), (rows, features, classes, dtype)
+    assert after == 1 or (before == 0 and not any(gave_up)), (before, after, gave_up)
+    if gave_up[0]:
+        # what is ignored has no loss, whatever happened; the loss that is NaN has gradients that are
+        assert gave_up[1] and gave_up[2] and gave_up[3] and (got[0][y == -100] == 0).all()
+    print(rows, features, classes, dtype, gave_up, flush=True)
+    ran_out += gave_up[0]
+    C.lib.dk_linear_cross_entropy_wait_limit(0)
+    assert all(torch.equal(a, c) for a, c in zip(step(), want))      # the next call is none the worse
+    C.lib.dk_linear_cross_entropy_wait_limit(1)
+assert ran_out
+"""
+
+
+def test_waits_that_run_out_leave_nan_and_a_status():
+    """With a limit of a nanosecond the kernels give up where the tensor cores or the copies keep them waiting: every value is
+    then NaN or the right one, the status says so, and the process goes on.  Tiles of one SM and of two; the longer the sum
+    the longer the wait.  In a process of its own: the status stays."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    cases = [(64, 2 ** 20, 48, "bf16", {}), (300, 2 ** 15, 10000, "bf16", {}), (64, 2 ** 17, 48, "fp32", {}), (300, 2 ** 15, 1000, "fp32", dict(label_smoothing=0.1))]
+    code = WAITS % (os.path.join(root, "deformable-kernels_b200"), os.path.join(root, "tests"), cases)
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
+    assert out.returncode == 0, (out.stdout[-1000:], out.stderr[-2000:])
+    print(out.stdout)
