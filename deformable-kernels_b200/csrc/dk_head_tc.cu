@@ -35,7 +35,11 @@ using ring::smem_u32;
 namespace {
 
 __device__ int g_head_error;  // set when a bounded wait ran out
-constexpr unsigned long long kWaitLimit = 2000000000;  // nanoseconds
+// Nanoseconds.  The longest wait is the epilogue's for one sum: a step of 64 takes 0.235 us where nothing hides the loads' latency, so 2^26
+// features take 0.25 s (more are refused), and a sum of the gradients, whose steps split_products bounds by all tiles' steps over the number of
+// clusters, some 30 ms (2^17 steps: one row, gradients and weights of 180 GB).  fp32 sums are taken every eight steps.
+constexpr unsigned long long kWaitLimit = 2000000000;
+constexpr int kMostFeatures = 1 << 26;
 std::atomic<unsigned long long> g_wait_limit{kWaitLimit};
 
 constexpr int kBox = 64;                    // values per side of a TMA box
@@ -1187,6 +1191,7 @@ int forward(const void* x, const void* w, const void* b, const long long* y, voi
             size_t ws_bytes, cudaStream_t s) {
   // With a backward to come the logits have to be the ones that it will compute: where p is nearly one, p - 1 is the difference of the two.
   const ForwardPlan p = forward_plan(h.T, h.D, h.V, dtype, few_rows(h.T, dtype) && !saved);
+  if (PIECES == 1 && !p.few && h.D > kMostFeatures) return DK_ERR_UNSUPPORTED;
   if (!ws || ws_bytes < tc_forward_bytes(h.T, h.D, h.V, dtype)) return DK_ERR_WORKSPACE;
   char* m = (char*)ws;
   if (p.few) {
@@ -1217,6 +1222,7 @@ template <typename T, typename E, int PIECES>
 int backward(const void* up, const void* x, const void* w, const void* b, const long long* y, const void* saved, void* dx, void* dw,
              void* db, const Shape& h, int dtype, void* ws, size_t ws_bytes, cudaStream_t s) {
   const BackwardPlan p = backward_plan(h.T, h.D, h.V, dtype);
+  if (PIECES == 1 && h.D > kMostFeatures) return DK_ERR_UNSUPPORTED;
   if (!ws || ws_bytes < p.bytes) return DK_ERR_WORKSPACE;
   char* m = (char*)ws;
   const float* stat = (const float*)saved;

@@ -35,3 +35,12 @@ def test_sizes_whose_loops_would_pass_32_bits_are_refused(which, dtype):
 def test_more_logits_than_a_plan_can_count_are_refused(dtype):
     for rows, classes in ((MOST, MOST), (2 ** 30, 2 ** 27)):
         assert calls(rows, 1, classes, dtype) == (UNSUPPORTED, UNSUPPORTED)
+
+
+@pytest.mark.parametrize("dtype", [1, 3])
+def test_sums_too_long_for_the_limit_of_a_wait_are_refused(dtype):
+    """2^26 features: 2^20 steps of a quarter of a microsecond."""
+    assert calls(8, 2 ** 26 + 1, 2, dtype) == (UNSUPPORTED, UNSUPPORTED)
+    assert calls(8, 2 ** 26, 2, dtype) == (WORKSPACE, WORKSPACE)
+    assert calls(4, 2 ** 26 + 1, 2, dtype) == (WORKSPACE, UNSUPPORTED)     # a few rows without a backward have no such sums
+    assert calls(8, 2 ** 26 + 1, 2, 0) == (WORKSPACE, WORKSPACE)           # fp32 sums are taken every eight steps
