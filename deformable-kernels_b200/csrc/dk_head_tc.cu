@@ -401,6 +401,24 @@ __device__ __forceinline__ void product(unsigned d, uint64_t a, uint64_t b, unsi
   for (int q = 0; q < 4; ++q) mma_ss<CG>(d + at, a + (uint64_t)(q * step_a >> 4), b + (uint64_t)(q * step_b >> 4), idesc, !fresh || q > 0);
 }
 
+// lane j: the sum over the warp's lanes of v[j], in fixed order; every step halves the columns that a lane still has
+__device__ __forceinline__ float column_sum(const float (&v)[32], int lane) {
+  float r[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float mine = lane & 16 ? v[i + 16] : v[i], other = lane & 16 ? v[i] : v[i + 16];
+    r[i] = mine + __shfl_xor_sync(0xffffffffu, other, 16);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float mine = lane & o ? r[i + o] : r[i], other = lane & o ? r[i] : r[i + o];
+      r[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+    }
+  return r[0];
+}
+
 // 16 columns of both sums of an fp32 accumulator, added to v (set: stored)
 template <int BN>
 __device__ __forceinline__ void take_both(float* v, unsigned a, bool set) {
@@ -712,7 +730,17 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
               v[h][j] = live ? p * g : 0.0f;
             }
           }
-          float s0 = 0, s1 = 0;
+          // of dz as it is, not as the products take it; 16-bit types: while the copy of the tile is under way
+          auto sum_columns = [&] {
+            float* to = a.column_sums + (long long)(row_base >> 5) * a.classes;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = col_base + c0 + 32 * h + lane;
+              const float all = column_sum(v[h], lane);
+              if (c < a.classes) to[c] = all;
+            }
+          };
+          if (PIECES > 1 && a.column_sums) sum_columns();  // the pieces take v apart
 #pragma unroll
           for (int pc = 0; pc < PIECES; ++pc) {
             if (lane == 0) stores_have_read();
@@ -735,21 +763,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
             ring::fence_proxy_async();
             __syncwarp();
             if (lane == 0) store_box(&a.dz_out, stage, col_base + c0, row_base, pc);
-            if (a.column_sums) {
-              // two columns a lane, of dz as the products see it: rounded, with 32-bit sums
-#pragma unroll 8
-              for (int r = 0; r < 32; ++r) {
-                const float2 f = unpack<E>(lds4(staged(stage, r, lane >> 2) + (lane & 3) * 4));
-                s0 += f.x, s1 += f.y;
-              }
-            }
           }
-          if (a.column_sums) {
-            const int c = col_base + c0 + 2 * lane;
-            float* to = a.column_sums + (long long)(row_base >> 5) * a.classes + c;
-            if (c < a.classes) to[0] = s0;
-            if (c + 1 < a.classes) to[1] = s1;
-          }
+          if (PIECES == 1 && a.column_sums) sum_columns();
         }
       } else {
         const Product& p = it.product ? a.dx : a.dw;

@@ -102,3 +102,19 @@ def test_waits_that_run_out_leave_nan_and_a_status():
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
     assert out.returncode == 0, (out.stdout[-1000:], out.stderr[-2000:])
     print(out.stdout)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("rows, features, classes", [(40, 8, 5), (200, 8, 70), (300, 16, 300)])
+def test_bias_gradients_are_sums_of_unrounded_values(rows, features, classes, dtype):
+    """dz is rounded to 16 bits for the two products, not for the bias gradient: its errors are those of fp32 sums (the
+    bound of the same call in fp32) and one rounding of the result.  Few features keep the first below what a rounding of
+    every dz would add where a class's dz cancel."""
+    x, w, y, b, up = make(rows, features, classes, dtype, seed=rows)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    loss = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), leaves[2])
+    db, = torch.autograd.grad(loss, leaves[2:], up.to(DEV))
+    out, far = H.head(x.float(), w.float(), y, b.float(), up)
+    info = torch.finfo(H.DTYPES[dtype])
+    bound = far["db"] + info.eps / 2 * out["db"].abs() + info.smallest_normal * info.eps / 2
+    assert ((db.cpu().double() - out["db"]).abs() <= bound).all()
