@@ -1147,7 +1147,7 @@ BackwardPlan backward_plan(int T, int D, int V, int dtype) {
     const long long even = (long long)div_up(div_up(all, n), 256) * 256;
     side = even < all ? (int)even : all;
   }
-  p.dz = pick(p.tc, p.vc, D, pieces);
+  p.dz = pick(T, V, D, pieces);  // the forward's: p - 1 of a class that is nearly certain takes the same logits, bit by bit
   p.grad = pick_gradients(p.tc, p.vc, D, pieces);
   split_products(p, D, pieces);
   const bool lay = laid_out(D, dtype);

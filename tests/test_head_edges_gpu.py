@@ -118,3 +118,36 @@ def test_bias_gradients_are_sums_of_unrounded_values(rows, features, classes, dt
     info = torch.finfo(H.DTYPES[dtype])
     bound = far["db"] + info.eps / 2 * out["db"].abs() + info.smallest_normal * info.eps / 2
     assert ((db.cpu().double() - out["db"]).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("rows, classes, dtype", [(100, 3000, "bf16"), (100, 30000, "bf16"), (300, 20000, "bf16"), (2100, 70000, "bf16"), (70000, 2100, "fp16"),
+                                                  (100, 3000, "fp32"), (300, 20000, "fp32"), (2100, 24000, "fp32"), (24000, 2100, "fp32")])
+def test_gradients_of_losses_near_zero_in_every_tile_shape(rows, classes, dtype):
+    """1 - p of a class that is nearly certain is the difference of the forward's logits and the backward's, which have to be the
+    same to the last bit in every shape of tiles, in calls that are cut into pieces too.  Logits of up to 24: one that
+    was off by a single step (2^-20) would be 2^-20 / 1e-5 = 10 % of it.  Else the others' probabilities are off by the two
+    logits' errors, (64 + 8) 2^-23 24, and 1 - p by three roundings of one; 16-bit dz and results are rounded once each."""
+    gen = torch.Generator().manual_seed(rows)
+    lift = 11.5 + torch.tensor(float(classes)).log().item()
+    y = torch.arange(rows) % 7 * (classes // 7)
+    w = torch.randn(classes, 64, generator=gen) * 0.05
+    x = torch.randn(rows, 64, generator=gen) * 0.1 + lift * w[y] / w[y].square().sum(1, keepdim=True)
+    x, w = (t.to(H.DTYPES[dtype]).to(DEV) for t in (x, w))
+    y, b = y.to(DEV), torch.zeros(classes, dtype=x.dtype, device=DEV)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    loss = functions().linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], reduction="sum")
+    got = torch.autograd.grad(loss, leaves)
+    with torch.no_grad():
+        z = x.double() @ w.double().t()
+        lse = torch.logsumexp(z, 1)
+        dz = z.sub_(lse[:, None]).exp_()
+        dz[torch.arange(rows, device=DEV), y] = 0
+        rest = dz.sum(1)
+        assert 1e-6 < rest.min() and rest.max() < 1e-2
+        dz[torch.arange(rows, device=DEV), y] = -rest
+        u = 0.0 if dtype == "fp32" else torch.finfo(x.dtype).eps / 2
+        tol = 72 * 2.0 ** -23 * 24 * 2 + 2.0 ** -22 / rest.min().item() + 2.1 * u
+        for a, c in zip(got, (dz @ w.double(), dz.t() @ x.double(), dz.sum(0))):
+            assert (a.double() - c).norm() < tol * c.norm(), ((a.double() - c).norm() / c.norm()).item()
+    del z, dz
+    torch.cuda.empty_cache()
