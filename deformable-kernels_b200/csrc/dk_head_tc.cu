@@ -19,6 +19,7 @@
 // (1.46 Pflop/s, 83 %).  The clock is at 1.5 GHz under this load: power is the bound of large calls.
 // Small calls are launches and the latency of one tile: 10 us for a tile of 1280 features.
 
+#include <float.h>
 #include <math_constants.h>
 
 #include <atomic>
@@ -906,6 +907,7 @@ __device__ __forceinline__ void load_odd(T (&v)[8], const LayOut& l, long long a
       if (c + e >= l.width) v[e] = (T)0.0f;
   }
 }
+constexpr float kLargestBf16 = 3.3895314e38f;  // (2 - 2^-7) 2^127
 // [rows][width] -> PIECES planes [rows][8 per_row] of E: fp32 in three bf16 pieces, 16-bit rows on 16 bytes; eight values a lane, `lanes` lanes a row
 template <typename T, typename E, int PIECES>
 __device__ __forceinline__ void lay_out_row(const LayOut& l, long long r, int first, int stride, long long ignore) {
@@ -932,7 +934,8 @@ __device__ __forceinline__ void lay_out_row(const LayOut& l, long long r, int fi
         float left = as_float(v[e]);
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-          out[p][e] = (E)left;
+          // the last 2^-9 of fp32's range would round to infinity
+          out[p][e] = (E)(p == 0 && fabsf(left) <= FLT_MAX ? fminf(fmaxf(left, -kLargestBf16), kLargestBf16) : left);
           left -= as_float(out[p][e]);
         }
       }

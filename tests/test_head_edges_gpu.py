@@ -151,3 +151,34 @@ def test_gradients_of_losses_near_zero_in_every_tile_shape(rows, classes, dtype)
             assert (a.double() - c).norm() < tol * c.norm(), ((a.double() - c).norm() / c.norm()).item()
     del z, dz
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows", [12, 200])
+def test_fp32_values_at_the_end_of_the_range(rows):
+    """The largest fp32 values are finite as three bf16 pieces too.  x = +-max with w = +-2^-125 in features of their own: logits of
+    8 (1 - 2^-24), exact but for the last bit; one product a logit that is not zero."""
+    big, classes = torch.finfo(torch.float32).max, 6
+    x, w = torch.zeros(rows, 16), torch.zeros(classes, 16)
+    for c in range(classes):
+        w[c, c] = 2.0 ** -125
+    y = torch.arange(rows) % classes
+    x[torch.arange(rows), y] = big * (1 - 2 * (torch.arange(rows) // classes % 2)).float()
+    b = torch.zeros(classes)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w, b)]
+    loss = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), leaves[2], reduction="none")
+    grads = torch.autograd.grad(loss.mean() * 2.0 ** -10, leaves)
+    ref = [t.double().requires_grad_(True) for t in (x, w, b)]
+    want = torch.nn.functional.cross_entropy(ref[0] @ ref[1].t() + ref[2], y, reduction="none")
+    want_grads = torch.autograd.grad(want.mean() * 2.0 ** -10, ref)
+    # a logit of 8 is off by 2^-21, what follows by a few roundings
+    assert ((loss.cpu().double() - want).abs() <= 2.0 ** -20 + 2.0 ** -21 * want).all()
+    # dz is off by that of itself and by three roundings of one (p - 1); a class's dz cancel in its bias gradient, their errors do not:
+    # the bound is of the sum of magnitudes
+    with torch.no_grad():
+        z = ref[0] @ ref[1].t()
+        dz = (torch.softmax(z, 1) - torch.nn.functional.one_hot(y, classes)).abs()
+        off = (2.0 ** -19 * dz + 2.0 ** -22) * (2.0 ** -10 / rows)
+        for a, c, bound in zip(grads[1:], want_grads[1:], (off.t() @ ref[0].abs(), off.sum(0))):
+            assert ((a.cpu().double() - c).abs() <= bound).all()
+    # w is of the size of fp32's smallest normal numbers, which a sum of less than that keeps to 2^-149
+    assert (grads[0].cpu().double() - want_grads[0]).abs().max() <= 2.0 ** -125 * 2.0 ** -8
