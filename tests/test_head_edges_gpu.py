@@ -3,6 +3,7 @@ second derivatives, waits that run out."""
 import pytest
 import torch
 
+import head_fp32 as F
 import head_oracle as H
 from test_head_gpu import DEV, check, functions, make, no_wait_ran_out  # noqa: F401  (the fixture watches every test)
 
@@ -182,3 +183,18 @@ def test_fp32_values_at_the_end_of_the_range(rows):
             assert ((a.cpu().double() - c).abs() <= bound).all()
     # w is of the size of fp32's smallest normal numbers, which a sum of less than that keeps to 2^-149
     assert (grads[0].cpu().double() - want_grads[0]).abs().max() <= 2.0 ** -125 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("t, d, v", F.SIZES)
+def test_fp32_keeps_24_bits_of_every_operand(t, d, v):
+    for scale, names in ((2.0, ("loss",)), (2.0 ** -6, ("dx", "dw"))):
+        x, w, y, b = F.case(t, d, v, scale)
+        out, far = F.bounds(x, w, y, b)
+        leaves = [t.to(DEV).requires_grad_(True) for t in (x, w)]
+        loss = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), b.to(DEV), reduction="sum")
+        got = dict(zip(("loss", "dx", "dw"), (loss.detach(),) + torch.autograd.grad(loss, leaves)))
+        with torch.no_grad():
+            got["alone"] = functions().linear_cross_entropy(x.to(DEV), w.to(DEV), y.to(DEV), b.to(DEV), reduction="sum")
+        out["alone"], far["alone"] = out["loss"], far["loss"]
+        for name in names + ("alone",) * (scale == 2.0):
+            assert ((got[name].cpu().double() - out[name]).abs() <= far[name]).all(), name
