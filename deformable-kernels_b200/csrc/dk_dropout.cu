@@ -298,6 +298,9 @@ extern "C" int dk_dropout(const void* input, void* output, long long count, long
                           unsigned long long offset, const void* state, void* used, int dtype, void* stream) {
   if (!input || !output || count <= 0 || run <= 0 || !(p >= 0.0 && p <= 1.0) || (used && !state)) return DK_ERR_BAD_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(state) | reinterpret_cast<uintptr_t>(used)) & 7) return DK_ERR_BAD_ARGUMENT;
+  // every block reads `state`, one of them writes `used`
+  const uintptr_t from = reinterpret_cast<uintptr_t>(state), to = reinterpret_cast<uintptr_t>(used);
+  if (used && from < to + 16 && to < from + 16) return DK_ERR_BAD_ARGUMENT;
   DropArgs a = {};
   a.count = (unsigned long long)count, a.run = (unsigned long long)run;
   a.seed = seed, a.offset = offset;

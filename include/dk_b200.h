@@ -292,7 +292,7 @@ int dk_offset_clip_backward(const void *grad_output, const void *offsets, const 
  * state: device, two 64-bit words (seed, offset) read by the kernel, so that a captured call draws anew when the caller
  * advances them; `offset` is added to the second, `seed` is not looked at; NULL: the arguments alone.  used: device, two
  * 64-bit words that receive the seed and offset of a call with `state` (what its backward passes as `state`, with offset 0),
- * or NULL.  0 <= p <= 1.  Dropped elements are zero whatever the input holds. */
+ * or NULL; it does not overlap `state`, nor `output` `input`.  0 <= p <= 1.  Dropped elements are zero whatever the input holds. */
 int dk_dropout(const void *input, void *output, long long count, long long run, double p, unsigned long long seed,
                unsigned long long offset, const void *state, void *used, int dtype, void *stream);
 

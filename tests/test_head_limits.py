@@ -44,3 +44,10 @@ def test_sums_too_long_for_the_limit_of_a_wait_are_refused(dtype):
     assert calls(8, 2 ** 26, 2, dtype) == (WORKSPACE, WORKSPACE)
     assert calls(4, 2 ** 26 + 1, 2, dtype) == (WORKSPACE, UNSUPPORTED)     # a few rows without a backward have no such sums
     assert calls(8, 2 ** 26 + 1, 2, 0) == (WORKSPACE, WORKSPACE)           # fp32 sums are taken every eight steps
+
+
+def test_dropout_does_not_write_the_state_that_it_reads():
+    from deformable_kernels import _cabi as C
+    at = ctypes.c_void_p
+    for state, used in ((64, 64), (64, 72), (64, 56)):
+        assert C.lib.dk_dropout(at(1024), at(2048), 8, 1, 0.5, 0, 0, at(state), at(used), 0, at(0)) == 1
