@@ -609,9 +609,10 @@ struct DropoutBackward : public Node {
     const c10::DeviceGuard guard(options.device());
     const Tensor dy = arrived_as(grads, sizes, options);
     Tensor dx = empty_as(dy, sizes);
-    check(lib.dk_dropout(cptr(dy), mptr(dx), dy.numel(), run, p, seed, on_device ? 0 : offset, cptr(used), nullptr, head_dtype_code(dy),
-                         stream_of(dy)),
-          "dropout backward");
+    if (dy.numel() > 0)
+      check(lib.dk_dropout(cptr(dy), mptr(dx), dy.numel(), run, p, seed, on_device ? 0 : offset, cptr(used), nullptr, head_dtype_code(dy),
+                           stream_of(dy)),
+            "dropout backward");
     return {dx};
   }
   std::string name() const override { return "DropoutFunctionBackward"; }
@@ -631,7 +632,7 @@ Tensor dropout(const Tensor& input, double p, const Tensor& state, unsigned long
     TORCH_CHECK_VALUE(state.numel() == 2, "the seed tensor holds two values, seed and offset");
   }
   const int code = head_dtype_code(input);
-  const bool grad = wants_grad({&input}) && input.numel() > 0;
+  const bool grad = wants_grad({&input});
   int64_t run = 1;
   for (int64_t d = input.dim() - shared_dims; d < input.dim(); ++d) run *= input.size(d);
   Tensor out, used;

@@ -198,3 +198,18 @@ def test_fp32_keeps_24_bits_of_every_operand(t, d, v):
         out["alone"], far["alone"] = out["loss"], far["loss"]
         for name in names + ("alone",) * (scale == 2.0):
             assert ((got[name].cpu().double() - out[name]).abs() <= far[name]).all(), name
+
+
+def test_dropout_of_nothing_has_a_gradient():
+    """An empty batch goes through a training step like any other."""
+    f = functions()
+    state = torch.tensor([3, 4], device=DEV)
+    for seed in (1, state):
+        x = torch.zeros(0, 8, device=DEV, requires_grad=True)
+        w = torch.ones(3, 8, device=DEV, requires_grad=True)
+        y = f.dropout(x, 0.5, seed)
+        assert y.requires_grad and y.shape == (0, 8)
+        dx, dw = torch.autograd.grad((y @ w.t()).sum(), [x, w])
+        assert dx.shape == (0, 8) and (dw == 0).all()
+        dx, = torch.autograd.grad(f.dropout(x, 0.5, seed).sum(), x)
+        assert dx.shape == (0, 8)
