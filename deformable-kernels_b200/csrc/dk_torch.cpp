@@ -594,30 +594,47 @@ inline Tensor arrived_as(const variable_list& grads, at::IntArrayRef sizes, cons
   return g.to(options.dtype()).contiguous();
 }
 
-struct DropoutBackward : public Node {
-  Tensor used;  // seed and offset of the forward call, where they came from the device; not visible outside
-  bool on_device = false;
-  unsigned long long seed = 0, offset = 0;
+// which elements a call dropped
+struct DropoutDraw {
+  Tensor used;  // seed and offset, where they came from the device; not visible outside
+  unsigned long long seed = 0, offset = 0;  // else
   double p = 0;
   int64_t run = 1;
+};
+void record_dropout(Tensor& out, const Tensor& from, const DropoutDraw& draw);
+
+struct DropoutBackward : public Node {
+  DropoutDraw draw;
+  bool on_device = false;
   std::vector<int64_t> sizes;
   at::TensorOptions options;
 
   variable_list apply(variable_list&& grads) override {
+    // the map is linear: the derivative of its gradient is the same map
+    const bool again = at::GradMode::is_enabled() && grads[0].defined() && grads[0].requires_grad();
     at::NoGradGuard no_grad;
-    TORCH_CHECK(!on_device || used.defined(), "Trying to backward through the graph a second time");
+    TORCH_CHECK(!on_device || draw.used.defined(), "Trying to backward through the graph a second time");
     const c10::DeviceGuard guard(options.device());
     const Tensor dy = arrived_as(grads, sizes, options);
     Tensor dx = empty_as(dy, sizes);
     if (dy.numel() > 0)
-      check(lib.dk_dropout(cptr(dy), mptr(dx), dy.numel(), run, p, seed, on_device ? 0 : offset, cptr(used), nullptr, head_dtype_code(dy),
-                           stream_of(dy)),
+      check(lib.dk_dropout(cptr(dy), mptr(dx), dy.numel(), draw.run, draw.p, draw.seed, on_device ? 0 : draw.offset, cptr(draw.used),
+                           nullptr, head_dtype_code(dy), stream_of(dy)),
             "dropout backward");
+    if (again) record_dropout(dx, grads[0], draw);
     return {dx};
   }
   std::string name() const override { return "DropoutFunctionBackward"; }
-  void release_variables() override { used.reset(); }
+  void release_variables() override { draw.used.reset(); }
 };
+
+void record_dropout(Tensor& out, const Tensor& from, const DropoutDraw& draw) {
+  auto node = std::make_shared<DropoutBackward>();
+  node->set_next_edges(collect_next_edges(from));
+  node->draw = draw, node->on_device = draw.used.defined();
+  node->sizes = out.sizes().vec(), node->options = out.options();
+  torch::autograd::set_history(out, node);
+}
 
 // `state`: [seed, offset] on the device, or undefined: the two numbers
 Tensor dropout(const Tensor& input, double p, const Tensor& state, unsigned long long seed, unsigned long long offset,
@@ -635,7 +652,8 @@ Tensor dropout(const Tensor& input, double p, const Tensor& state, unsigned long
   const bool grad = wants_grad({&input});
   int64_t run = 1;
   for (int64_t d = input.dim() - shared_dims; d < input.dim(); ++d) run *= input.size(d);
-  Tensor out, used;
+  Tensor out;
+  DropoutDraw draw = {Tensor(), seed, offset, p, run};
   {
     at::NoGradGuard no_grad;
     const c10::DeviceGuard guard(input.device());
@@ -643,18 +661,12 @@ Tensor dropout(const Tensor& input, double p, const Tensor& state, unsigned long
     out = empty_as(x, x.sizes());
     if (x.numel() > 0) {
       const Tensor st = state.defined() ? state.contiguous() : Tensor();
-      if (grad && st.defined()) used = empty_of(x, {2}, at::kLong);
-      check(lib.dk_dropout(cptr(x), mptr(out), x.numel(), run, p, seed, offset, cptr(st), mptr(used), code, stream_of(x)), "dropout forward");
+      if (grad && st.defined()) draw.used = empty_of(x, {2}, at::kLong);
+      check(lib.dk_dropout(cptr(x), mptr(out), x.numel(), run, p, seed, offset, cptr(st), mptr(draw.used), code, stream_of(x)),
+            "dropout forward");
     }
   }
-  if (grad) {
-    auto node = std::make_shared<DropoutBackward>();
-    node->set_next_edges(collect_next_edges(input));
-    node->used = used, node->on_device = used.defined();
-    node->seed = seed, node->offset = offset, node->p = p, node->run = run;
-    node->sizes = out.sizes().vec(), node->options = out.options();
-    torch::autograd::set_history(out, node);
-  }
+  if (grad) record_dropout(out, input, draw);
   return out;
 }
 

@@ -213,3 +213,21 @@ def test_dropout_of_nothing_has_a_gradient():
         assert dx.shape == (0, 8) and (dw == 0).all()
         dx, = torch.autograd.grad(f.dropout(x, 0.5, seed).sum(), x)
         assert dx.shape == (0, 8)
+
+
+def test_second_derivatives_through_dropout():
+    """The gradient of a gradient goes through the mask as well: d/dx of |d/dx (sum of squares of what is kept)|^2."""
+    f = functions()
+    state = torch.tensor([3, 4], device=DEV)
+    for seed in (7, state):
+        x = torch.randn(40, 16, device=DEV, dtype=torch.double, requires_grad=True)
+        keep = (f.dropout(torch.ones_like(x), 0.25, seed) != 0).detach()
+        outcomes = []
+        for drop in (lambda t: f.dropout(t, 0.25, seed), lambda t: torch.where(keep, t / 0.75, torch.zeros_like(t))):
+            dx, = torch.autograd.grad(drop(x).pow(3).sum(), x, create_graph=True)
+            assert dx.requires_grad
+            ddx, = torch.autograd.grad(dx.square().sum(), x, create_graph=True)
+            dddx, = torch.autograd.grad(ddx.square().sum(), x)
+            outcomes.append((dx.detach(), ddx.detach(), dddx))
+        for a, c in zip(*outcomes):
+            assert torch.allclose(a, c, rtol=1e-13, atol=0)
