@@ -682,6 +682,15 @@ inline Tensor aligned(const Tensor& t) {
   return reinterpret_cast<uintptr_t>(c.const_data_ptr()) & 15 ? c.clone() : c;
 }
 
+// what gradients that were asked for with create_graph=True hang on
+struct NoSecondDerivative : public Node {
+  variable_list apply(variable_list&&) override {
+    TORCH_CHECK_NOT_IMPLEMENTED(false, "linear_cross_entropy has no second derivative");
+    return {};
+  }
+  std::string name() const override { return "LinearCrossEntropyFunctionNoSecondDerivative"; }
+};
+
 struct LinearCrossEntropyBackward : public Node {
   SavedVariable input, weight, bias, target;
   Tensor saved;  // what the rows' probabilities are made of, and their count; not visible outside
@@ -690,6 +699,17 @@ struct LinearCrossEntropyBackward : public Node {
   std::vector<int64_t> in_sizes, out_sizes;
 
   variable_list apply(variable_list&& grads) override {
+    if (!at::GradMode::is_enabled()) return gradients(grads);
+    variable_list out = gradients(grads);
+    auto node = std::make_shared<NoSecondDerivative>();
+    auto edges = next_edges();
+    for (auto& e : collect_next_edges(grads)) edges.push_back(e);
+    node->set_next_edges(std::move(edges));
+    for (Tensor& t : out)
+      if (t.defined()) torch::autograd::set_history(t, node);
+    return out;
+  }
+  variable_list gradients(const variable_list& grads) {
     at::NoGradGuard no_grad;
     const Tensor x = input.unpack(), w = weight.unpack(), y = target.unpack(), b = has_bias ? bias.unpack() : Tensor();
     TORCH_CHECK(saved.defined(), "Trying to backward through the graph a second time");

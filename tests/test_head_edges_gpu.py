@@ -231,3 +231,26 @@ def test_second_derivatives_through_dropout():
             outcomes.append((dx.detach(), ddx.detach(), dddx))
         for a, c in zip(*outcomes):
             assert torch.allclose(a, c, rtol=1e-13, atol=0)
+
+
+def test_second_derivatives_of_the_loss_are_refused():
+    """Its gradients are no constants: a term made of them raises instead of having no derivative."""
+    x, w, y, b, up = (t.to(DEV) for t in make(20, 16, 30, "fp32", seed=2))
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(functions().linear_cross_entropy(x, w, y, b), leaves)
+    loss = functions().linear_cross_entropy(x, w, y, b)
+    got = torch.autograd.grad(loss, leaves, create_graph=True)
+    assert all(torch.equal(a, c) and a.requires_grad for a, c in zip(got, want))
+    for g in got:
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(g.square().sum(), leaves, retain_graph=True, allow_unused=True)
+    loss = functions().linear_cross_entropy(x, w, y, b, reduction="none")
+    up = torch.ones(20, device=DEV, requires_grad=True)
+    dx, = torch.autograd.grad(loss, x, up, create_graph=True)
+    with pytest.raises(NotImplementedError):
+        torch.autograd.grad(dx.sum(), up)
+    # asked for and not used: as without it
+    functions().linear_cross_entropy(x, w, y, b).backward(create_graph=True)
+    assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1]) and torch.equal(b.grad, want[2])
+    for t in leaves:
+        t.grad = None
