@@ -40,7 +40,7 @@ class LinearCrossEntropy(nn.Linear):
 
     ``features`` [..., in_features], ``target`` [...] int64.  Parameters, initialisation and state dict are those of
     ``nn.Linear(in_features, num_classes, bias)``; ``ignore_index``, ``reduction`` and ``label_smoothing`` those of
-    ``nn.CrossEntropyLoss``.  Under autocast the features are taken in its dtype."""
+    ``nn.CrossEntropyLoss``.  Under autocast the features are taken in its dtype, but for float64, which autocast leaves alone."""
 
     def __init__(self, in_features, num_classes, bias=True, dropout=0.0, ignore_index=-100, reduction='mean', label_smoothing=0.0,
                  device=None, dtype=None):
@@ -54,7 +54,7 @@ class LinearCrossEntropy(nn.Linear):
         input = self.dropout(input)
         if target is None:
             return nn.functional.linear(input, self.weight, self.bias)
-        if input.is_cuda and torch.is_autocast_enabled():
+        if input.is_cuda and torch.is_autocast_enabled() and input.dtype != torch.float64:
             input = input.to(torch.get_autocast_dtype('cuda'))
         return linear_cross_entropy(input, self.weight, target, self.bias, self.ignore_index, self.reduction, self.label_smoothing)
 

@@ -254,3 +254,15 @@ def test_second_derivatives_of_the_loss_are_refused():
     assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1]) and torch.equal(b.grad, want[2])
     for t in leaves:
         t.grad = None
+
+
+def test_autocast_leaves_fp64_alone():
+    from deformable_kernels.modules import LinearCrossEntropy
+    torch.manual_seed(1)
+    head = LinearCrossEntropy(20, 7).to(DEV, torch.float64)
+    x, y = torch.randn(30, 20, device=DEV, dtype=torch.float64), torch.randint(0, 7, (30,), device=DEV)
+    want = head(x, y)
+    for dtype in (torch.float16, torch.bfloat16):
+        with torch.autocast("cuda", dtype=dtype):
+            got = head(x, y)
+        assert got.dtype == torch.float64 and torch.equal(got, want)
