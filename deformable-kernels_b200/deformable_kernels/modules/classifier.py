@@ -15,8 +15,8 @@ __all__ = ['Dropout', 'LinearCrossEntropy']
 class Dropout(nn.Module):
     """``nn.Dropout`` without a stored mask.  Each call in training mode draws its generator's seed and offset on the device
     from torch's default CUDA generator: ``torch.manual_seed`` repeats the masks, activation checkpointing makes the same
-    one again, and a captured call draws anew at every replay.  ``shared_dims``: the elements of that many trailing
-    dimensions are dropped together (2: whole feature planes)."""
+    one again, and a captured call draws anew at every replay.  The result has the input's memory format.  ``shared_dims``: the
+    elements of that many trailing dimensions are dropped together (2: whole feature planes)."""
 
     def __init__(self, p=0.5, shared_dims=0):
         super().__init__()
@@ -29,7 +29,18 @@ class Dropout(nn.Module):
         if not self.training or self.p == 0:
             return input
         state = torch.randint(0, 2 ** 63 - 1, (2,), device=input.device)
-        return dropout(input, self.p, state, shared_dims=self.shared_dims)
+        if input.is_contiguous():
+            return dropout(input, self.p, state, shared_dims=self.shared_dims)
+        # dense in another order (channels last): the draws are independent, so they can follow the memory, except that the
+        # elements which share one have to be neighbours there
+        order = sorted(range(input.dim()), key=input.stride, reverse=True)
+        back = sorted(range(input.dim()), key=order.__getitem__)
+        moved = input.permute(order)
+        if not moved.is_contiguous():
+            return dropout(input, self.p, state, shared_dims=self.shared_dims)
+        if min(order[input.dim() - self.shared_dims:], default=input.dim()) >= input.dim() - self.shared_dims:
+            return dropout(moved, self.p, state, shared_dims=self.shared_dims).permute(back)
+        return dropout(input, self.p, state, shared_dims=self.shared_dims).permute(order).contiguous().permute(back)
 
     def extra_repr(self):
         return 'p={}, shared_dims={}'.format(self.p, self.shared_dims)

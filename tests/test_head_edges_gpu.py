@@ -266,3 +266,28 @@ def test_autocast_leaves_fp64_alone():
         with torch.autocast("cuda", dtype=dtype):
             got = head(x, y)
         assert got.dtype == torch.float64 and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("shared", [0, 1, 2, 3])
+def test_dropout_module_keeps_the_memory_format(shared):
+    """As nn.Dropout does: channels last, transposed batches, planes of a permuted batch; elements that share a draw still do."""
+    from deformable_kernels.modules import Dropout
+    m = Dropout(0.4, shared_dims=shared)
+    base = torch.randn(12, 10, 9, 7, device=DEV)
+    views = [base, base.contiguous(memory_format=torch.channels_last), base.transpose(0, 1), base.permute(3, 1, 0, 2), base.permute(1, 0, 3, 2),
+             base[:, :1].contiguous(memory_format=torch.channels_last), base[:, :, 2:], base[:1].expand(12, 10, 9, 7)]
+    for x in views:
+        x = x.detach().requires_grad_(True)
+        torch.manual_seed(3)
+        y = m(x)
+        stock = torch.nn.functional.dropout(x, 0.4)
+        # (the stride of a dimension of size one addresses nothing)
+        assert y.shape == x.shape and all(a == c or n == 1 for a, c, n in zip(y.stride(), stock.stride(), x.shape))
+        keep = y.detach() != 0
+        assert torch.equal(y.detach(), torch.where(keep, x.detach() * (1 / 0.6), torch.zeros_like(x)))
+        runs = keep.reshape(*x.shape[:4 - shared], -1)
+        assert shared == 0 or torch.equal(runs.all(-1), runs.any(-1))
+        share = runs[..., 0].float().mean().item()
+        assert abs(share - 0.6) < 5 * (0.24 / runs[..., 0].numel()) ** 0.5
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert torch.equal(dx != 0, keep)
