@@ -8,6 +8,7 @@
 // tile.  An operand is K-major (rows of the tensor are rows of the product) or MN-major (columns are); both
 // come as boxes of 64 x 64 values, 128 swizzled bytes a row.
 //
+// 16-bit sums stay in TMEM, those of the logits up to 4096 features (kLongDepth).
 // fp32 operands are three bf16 pieces each (8 bits a piece, 24 in all).  A stage holds one piece of both; the six products of
 // pieces that reach 2^-24 are taken from three stages, that of the leading pieces into one accumulator, the five
 // small ones into another: the additions of the tensor cores cut, and a cut of the small sum costs nothing.  After every eight steps
@@ -432,9 +433,26 @@ __device__ __forceinline__ void take_both(float* v, unsigned a, bool set) {
   for (int j = 0; j < 16; ++j) v[j] = set ? lead[j] + small[j] : v[j] + (lead[j] + small[j]);
 }
 
+// the same where there is one sum
+__device__ __forceinline__ void take_one(float* v, unsigned a, bool set) {
+  float sum[16];
+  ld16(sum, a);
+  wait_ld(sum);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = set ? sum[j] : v[j] + sum[j];
+}
+
 // ---- the kernel
 
-template <int CG, int BN, int ROLE, typename E, int PIECES>
+// 16-bit logits: an addition of the tensor cores cuts, so the error of a sum in TMEM grows with its length (losses of 1024 rows, 1000 classes, bf16
+// features: 4.7e-7 of themselves at 1024 features, 1.1e-6 at 2560, 1.8e-6 at 4096, 7.8e-6 at 16384, 1.2e-4 at 262144).  Above 4096 features the sum is added up in
+// registers every 2048 (9e-7 at 16384); that costs up to a fifth of the time of many tiles (4096 rows, 4096 features, 21841 classes: loss 458 -> 540 us, step
+// 2.34 -> 2.49 ms; at 2560 features it would be 300 -> 355 and 1.43 -> 1.64), and 1 to 3 % of few (1024 x 16384 x 1000).
+constexpr int kLongDepth = 64, kLongChunk = 32;  // steps of 64 features
+static_assert(kLongDepth >= kLongChunk, "the last sum is taken by itself: there is one before it");
+
+// LONG: many features, whose sums are added up in registers every kLongChunk steps
+template <int CG, int BN, int ROLE, typename E, int PIECES, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) unsigned char smem[];
   constexpr int kStage = stage_bytes<CG, BN>();
@@ -442,7 +460,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
   constexpr int kGroups = BN >= 128 ? 2 : 1;       // epilogue warps side by side
   constexpr int kWide = BN / kGroups;              // columns of an epilogue warp
   constexpr int kAcc = PIECES == 1 ? BN : 2 * BN;  // columns of an accumulator
-  constexpr int kChunk = PIECES == 1 ? 1 << 30 : 8;  // steps between two takings of the accumulator
+  constexpr bool kTaken = PIECES > 1 || LONG;      // sums in registers
+  constexpr int kChunk = PIECES > 1 ? 8 : LONG ? kLongChunk : 1 << 30;  // steps between two takings of the accumulator
   static_assert(PIECES == 1 || kWide == 64, "the sums of a row are 64 registers");
   static_assert(2 * kAcc <= 512, "two accumulators in TMEM");
   SharedTail& t = *reinterpret_cast<SharedTail*>(smem + kStages * kStage + 8 * kStageWarp);
@@ -633,26 +652,31 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
       // the row's own class as a column of this warp, -1: elsewhere
       const long long far = y - a.class0 - col_base;
       const int own = far >= 0 && far < kWide ? (int)far : -1;
-      const int b = round & 1;
-      const unsigned d = tmem + lanes + b * kAcc + grp * kWide;
-      float got[PIECES == 1 ? 1 : 2][32];  // fp32: the sums
+      float got[kTaken ? kWide / 32 : 1][32];  // the sums that have left TMEM
       bool gone = false;  // the products never came: what the tile leaves is NaN
-      if (PIECES == 1) {
-        gone = wait(smem_u32(&t.acc_full[b]), (round >> 1) & 1, abort_flag, a.wait_limit);
-        tc::fence_after();
-        ++round;
-      } else {
-        for (int k = 0; k < it.count; k += kChunk, ++round) {
+      if (kTaken) {
+        // fp32: all of them; else all but the last
+        for (int k = 0; PIECES > 1 ? k < it.count : k + kChunk < it.count; k += kChunk, ++round) {
           const int bk = round & 1;
           gone |= wait(smem_u32(&t.acc_full[bk]), (round >> 1) & 1, abort_flag, a.wait_limit);
           tc::fence_after();
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
+          for (int h = 0; h < (kTaken ? kWide / 16 : 0); ++h) {
             __syncwarp();
-            take_both<BN>(&got[PIECES == 1 ? 0 : h >> 1][(h & 1) * 16], tmem + lanes + bk * kAcc + grp * kWide + 16 * h, k == 0);
+            float* sums = &got[h >> 1][(h & 1) * 16];
+            const unsigned from = tmem + lanes + bk * kAcc + grp * kWide + 16 * h;
+            if (PIECES == 1) take_one(sums, from, k == 0);
+            else take_both<BN>(sums, from, k == 0);
           }
           release(bk);
         }
+      }
+      const int b = round & 1;
+      const unsigned d = tmem + lanes + b * kAcc + grp * kWide;
+      if (PIECES == 1) {
+        gone |= wait(smem_u32(&t.acc_full[b]), (round >> 1) & 1, abort_flag, a.wait_limit);
+        tc::fence_after();
+        ++round;
       }
       const float g = !gone && y >= 0 && y < a.all_classes ? now.up * unit : CUDART_NAN_F;  // of a live row
       const float factor = gone ? CUDART_NAN_F : back;
@@ -662,14 +686,15 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           __syncwarp();
           ld32(v, d + c);
           wait_ld(v);
-        } else {
+        }
+        if (kTaken) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = c == 0 ? got[0][j] : got[PIECES == 1 ? 0 : 1][j];
+          for (int j = 0; j < 32; ++j) v[j] = PIECES == 1 ? v[j] + got[kTaken ? c >> 5 : 0][j] : got[kTaken ? c >> 5 : 0][j];
         }
       };
       if (ROLE == kStats) {
         float top = -CUDART_INF_F, sum = 0, all = 0, picked = 0;
-#pragma unroll(PIECES == 1 ? 1 : 2)
+#pragma unroll(kTaken ? kWide / 32 : 1)
         for (int c0 = 0; c0 < kWide; c0 += 32) {
           float z[32];
           columns(z, c0);
@@ -709,7 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
           if (own >= 0 && own + col_base < a.classes) a.picked[row] = picked;
         }
       } else if (ROLE == kDz) {
-#pragma unroll 1
+#pragma unroll(kTaken ? kWide / kBox : 1)
         for (int c0 = 0; c0 < kWide; c0 += kBox) {
           const bool inside = row_base < a.rows && col_base + c0 < a.classes;
           if (!inside) break;  // of the whole warp
@@ -1040,7 +1065,9 @@ int clusters_of(const Config& c) { return device_sm_count() / c.cg; }
 
 template <int CG, int BN, int ROLE, typename E, int PIECES>
 int launch_one(const Args& a, int items, cudaStream_t s) {
-  auto kernel = head_kernel<CG, BN, ROLE, E, PIECES>;
+  auto kernel = head_kernel<CG, BN, ROLE, E, PIECES, false>;
+  if constexpr (PIECES == 1 && ROLE != kGrad)
+    if (a.depth > kLongDepth) kernel = head_kernel<CG, BN, ROLE, E, PIECES, true>;
   const int rc = enable_smem(kernel, smem_bytes<CG, BN>());
   if (rc != DK_OK) return rc;
   const int clusters = device_sm_count() / CG;

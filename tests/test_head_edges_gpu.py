@@ -291,3 +291,37 @@ def test_dropout_module_keeps_the_memory_format(shared):
         assert abs(share - 0.6) < 5 * (0.24 / runs[..., 0].numel()) ** 0.5
         dx, = torch.autograd.grad(y, x, torch.ones_like(y))
         assert torch.equal(dx != 0, keep)
+
+
+@pytest.mark.parametrize("rows, features, classes, dtype", [(64, 2 ** 18, 90, "bf16"), (64, 2 ** 18, 90, "fp16"), (300, 2 ** 16 + 8, 9500, "bf16"), (4, 2 ** 18, 90, "bf16"),
+                                                            (40, 2 ** 17 + 3, 64, "bf16"), (150, 4160, 19000, "fp16"), (64, 2 ** 18, 90, "fp32")])
+def test_long_sums_of_one_sign(rows, features, classes, dtype):
+    """Logits whose products all have the same sign: the tensor cores' additions cut, always downwards.  In registers every 2048
+    features (128 additions of 2^-23 at most, then one of 2^-24 each), the sum keeps its precision however long it is."""
+    gen = torch.Generator(device=DEV).manual_seed(features)
+    share = torch.linspace(0, 1, classes, device=DEV)[:, None]
+    w = (torch.rand(1, features, generator=gen, device=DEV) + 0.5) * share * (8.0 / features)
+    x = torch.rand(rows, features, generator=gen, device=DEV) + 0.5
+    if dtype == "fp16":
+        w, x = w * 256, x / 256      # out of the subnormal numbers
+    x, w = (t.to(H.DTYPES[dtype]) for t in (x, w))
+    y = torch.arange(rows, device=DEV) % 2       # among the smallest logits: the loss is that of the largest
+    z = torch.cat([x.double() @ part.double().t() for part in w.split(1000)], 1)
+    lse = torch.logsumexp(z, 1)
+    want = lse - z.gather(1, y[:, None]).squeeze(1)
+    additions = (128 + features // 2048 / 2) * 2.0 ** -23
+    tol = 2 * additions * z.amax(1) + 2.0 ** -20 * (1 + lse)
+    with torch.no_grad():
+        alone = functions().linear_cross_entropy(x, w, y, reduction="none")
+    x.requires_grad_(True)
+    loss = functions().linear_cross_entropy(x, w, y, reduction="none")
+    dx, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    assert ((loss.detach().double() - want).abs() <= tol).all(), ((loss.detach().double() - want).abs() / tol).max().item()
+    assert ((alone.double() - want).abs() <= tol).all()
+    # and the backward's logits are the same: the gradients are theirs
+    dz = torch.exp(z - lse[:, None])
+    dz[torch.arange(rows, device=DEV), y] -= 1
+    want_dx = sum(dz[:, i:i + 1000] @ w[i:i + 1000].double() for i in range(0, classes, 1000))
+    u = torch.finfo(x.dtype).eps / 2
+    mag = sum(dz[:, i:i + 1000].abs() @ w[i:i + 1000].double().abs() for i in range(0, classes, 1000))
+    assert ((dx.double() - want_dx).abs() <= (2 * tol.max() + u + (classes + 16) * 2.0 ** -23) * mag + u * want_dx.abs() + torch.finfo(x.dtype).smallest_normal).all()
