@@ -37,11 +37,9 @@ using ring::smem_u32;
 namespace {
 
 __device__ int g_head_error;  // set when a bounded wait ran out
-// Nanoseconds.  The longest wait is the epilogue's for one sum: a step of 64 takes 0.235 us where nothing hides the loads' latency, so 2^26
-// features take 0.25 s (more are refused), and a sum of the gradients, whose steps split_products bounds by all tiles' steps over the number of
-// clusters, some 30 ms (2^17 steps: one row, gradients and weights of 180 GB).  fp32 sums are taken every eight steps.
+// Nanoseconds.  The longest wait is the epilogue's for one sum in TMEM: 1024 steps of a gradient (split_products), 64 of the logits (kLongDepth), 8 of
+// fp32 with six products each.  A step takes 0.235 us where nothing hides the loads' latency: a quarter of a millisecond.
 constexpr unsigned long long kWaitLimit = 2000000000;
-constexpr int kMostFeatures = 1 << 26;
 std::atomic<unsigned long long> g_wait_limit{kWaitLimit};
 
 constexpr int kBox = 64;                    // values per side of a TMA box
@@ -1131,8 +1129,12 @@ void split_products(BackwardPlan& p, int D, int pieces) {
   const long long total = tiles_w * blocks_w + tiles_x * blocks_x;
   // at least 32 steps a split (of fp32, six products each, 8): the launch that joins the sums takes as long as some 20 steps
   const int least = pieces == 1 ? 32 : 8;
+  // and of 16-bit types at most 1024, 4096 additions that cut: 2^-12 of a sum of one sign, half of what fp16 rounds.  Parts of sums are rounded additions; they
+  // take 8 KB of scratch a feature at most (a piece has 2^27 values of dz).
+  constexpr long long kMostSteps = 1024;
   long long per = total / clusters + 1;
   if (per < least) per = least;
+  if (pieces == 1 && per > kMostSteps) per = kMostSteps;
   p.per_w = (int)(per < blocks_w ? per : blocks_w), p.per_x = (int)(per < blocks_x ? per : blocks_x);
   p.splits_w = div_up(blocks_w, p.per_w), p.splits_x = div_up(blocks_x, p.per_x);
   p.per_w = div_up(blocks_w, p.splits_w), p.per_x = div_up(blocks_x, p.splits_x);
@@ -1236,7 +1238,6 @@ int forward(const void* x, const void* w, const void* b, const long long* y, voi
             size_t ws_bytes, cudaStream_t s) {
   // With a backward to come the logits have to be the ones that it will compute: where p is nearly one, p - 1 is the difference of the two.
   const ForwardPlan p = forward_plan(h.T, h.D, h.V, dtype, few_rows(h.T, dtype) && !saved);
-  if (PIECES == 1 && !p.few && h.D > kMostFeatures) return DK_ERR_UNSUPPORTED;
   if (!ws || ws_bytes < tc_forward_bytes(h.T, h.D, h.V, dtype)) return DK_ERR_WORKSPACE;
   char* m = (char*)ws;
   if (p.few) {
@@ -1267,7 +1268,6 @@ template <typename T, typename E, int PIECES>
 int backward(const void* up, const void* x, const void* w, const void* b, const long long* y, const void* saved, void* dx, void* dw,
              void* db, const Shape& h, int dtype, void* ws, size_t ws_bytes, cudaStream_t s) {
   const BackwardPlan p = backward_plan(h.T, h.D, h.V, dtype);
-  if (PIECES == 1 && h.D > kMostFeatures) return DK_ERR_UNSUPPORTED;
   if (!ws || ws_bytes < p.bytes) return DK_ERR_WORKSPACE;
   char* m = (char*)ws;
   const float* stat = (const float*)saved;

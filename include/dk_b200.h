@@ -305,8 +305,7 @@ int dk_dropout(const void *input, void *output, long long count, long long run, 
  * float (double for DK_F64).  saved: 2 rows + 2 values that the backward takes back, or
  * NULL.  input, weight,
  * their gradients and the workspace begin on 16 bytes.  Any gradient may be NULL.
- * DK_ERR_UNSUPPORTED: a size above 2^31 - 65536, more than 2^56 logits, 16-bit tensors of more than 2^26
- * features (but for the loss alone of up to four rows). */
+ * DK_ERR_UNSUPPORTED: a size above 2^31 - 65536, more than 2^56 logits. */
 /* The kernels wait for their own copies and products only, and no wait goes on for ever: after two seconds (time for which the
  * process is suspended does not count) the kernel ends, what it could not compute is NaN (losses, gradients), and
  * dk_ring_error_status() says so.  dk_linear_cross_entropy_wait_limit sets that limit, in nanoseconds, for the calls

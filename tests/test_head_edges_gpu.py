@@ -98,7 +98,8 @@ def test_waits_that_run_out_leave_nan_and_a_status():
     import subprocess
     import sys
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    cases = [(64, 2 ** 20, 48, "bf16", {}), (300, 2 ** 15, 10000, "bf16", {}), (64, 2 ** 17, 48, "fp32", {}), (300, 2 ** 15, 1000, "fp32", dict(label_smoothing=0.1))]
+    cases = [(64, 4096, 48, "bf16", {}), (300, 4096, 10000, "bf16", {}), (2 ** 18, 2048, 128, "bf16", {}), (64, 2 ** 17, 48, "fp32", {}),
+             (300, 2 ** 15, 1000, "fp32", dict(label_smoothing=0.1))]
     code = WAITS % (os.path.join(root, "deformable-kernels_b200"), os.path.join(root, "tests"), cases)
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
     assert out.returncode == 0, (out.stdout[-1000:], out.stderr[-2000:])
@@ -325,3 +326,46 @@ def test_long_sums_of_one_sign(rows, features, classes, dtype):
     u = torch.finfo(x.dtype).eps / 2
     mag = sum(dz[:, i:i + 1000].abs() @ w[i:i + 1000].double().abs() for i in range(0, classes, 1000))
     assert ((dx.double() - want_dx).abs() <= (2 * tol.max() + u + (classes + 16) * 2.0 ** -23) * mag + u * want_dx.abs() + torch.finfo(x.dtype).smallest_normal).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_long_gradient_sums_of_one_sign(dtype):
+    """dw of 2^20 equal rows: without weights p is 1/8 and dz -7/8 or 1/8, exactly, so a class's gradient is a sum of equal terms.
+    At most 4096 additions of a sum cut (2^-23 each), its parts are rounded, the result is rounded once."""
+    rows, features, classes = 2 ** 20, 8192, 8
+    one = (torch.rand(features, generator=torch.Generator().manual_seed(1)) + 1).to(H.DTYPES[dtype]).to(DEV)
+    x = one.expand(rows, features).contiguous()
+    w = torch.zeros(classes, features, dtype=x.dtype, device=DEV, requires_grad=True)
+    y = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    loss = functions().linear_cross_entropy(x, w, y)
+    dw, = torch.autograd.grad(loss, w)
+    dz = torch.full((classes, 1), 0.125, dtype=torch.double, device=DEV)
+    dz[0] -= 1
+    tol = 4096 * 2.0 ** -23 + 300 * 2.0 ** -24 + torch.finfo(x.dtype).eps / 2
+    want = dz * one.double()
+    assert ((dw.double() - want).abs() <= tol * want.abs()).all(), ((dw.double() - want).abs() / want.abs()).max().item()
+    del x
+    torch.cuda.empty_cache()
+
+
+def test_features_in_the_millions():
+    """2^23 + 3 features (one bf16 row of 17 MB): the loss and its gradients against fp64."""
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    d = 2 ** 23 + 3
+    for rows in (2, 9):
+        x = (torch.randn(rows, d, generator=gen, device=DEV)).bfloat16()
+        w = (torch.randn(3, d, generator=gen, device=DEV) * 2.0 ** -11).bfloat16()
+        y = torch.arange(rows, device=DEV) % 3
+        leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+        loss = functions().linear_cross_entropy(x, w, y, reduction="none")
+        dx, dw = torch.autograd.grad(loss, leaves, torch.ones_like(loss))
+        xd, wd = x.detach().double(), w.detach().double()
+        z = xd @ wd.t()
+        want = torch.nn.functional.cross_entropy(z, y, reduction="none")
+        # sums of 2^23 random terms of 2^-11: magnitudes of 2^23 2^-11 2 / pi, of which 128 additions cut at a time; two logits a loss
+        off = 2 * (128 * 2.0 ** -23 * 2.0 ** 11 / 2048 + 4096 * 2.0 ** -24 * 4) + 2.0 ** -20
+        assert ((loss.detach().double() - want).abs() <= off * (1 + want)).all(), (loss.detach().double() - want).abs().max().item()
+        dz = torch.softmax(z, 1)
+        dz[torch.arange(rows), y] -= 1
+        for a, c in ((dx, dz @ wd), (dw, dz.t() @ xd)):
+            assert (a.double() - c).norm() <= (2.0 ** -7 + 4 * off) * c.norm()

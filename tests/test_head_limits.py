@@ -37,13 +37,10 @@ def test_more_logits_than_a_plan_can_count_are_refused(dtype):
         assert calls(rows, 1, classes, dtype) == (UNSUPPORTED, UNSUPPORTED)
 
 
-@pytest.mark.parametrize("dtype", [1, 3])
-def test_sums_too_long_for_the_limit_of_a_wait_are_refused(dtype):
-    """2^26 features: 2^20 steps of a quarter of a microsecond."""
-    assert calls(8, 2 ** 26 + 1, 2, dtype) == (UNSUPPORTED, UNSUPPORTED)
-    assert calls(8, 2 ** 26, 2, dtype) == (WORKSPACE, WORKSPACE)
-    assert calls(4, 2 ** 26 + 1, 2, dtype) == (WORKSPACE, UNSUPPORTED)     # a few rows without a backward have no such sums
-    assert calls(8, 2 ** 26 + 1, 2, 0) == (WORKSPACE, WORKSPACE)           # fp32 sums are taken every eight steps
+@pytest.mark.parametrize("dtype", range(4))
+def test_many_features_are_no_reason_to_refuse(dtype):
+    """No sum stays in one accumulator for longer than a wait may take."""
+    assert calls(8, 2 ** 28, 2, dtype) == (WORKSPACE, WORKSPACE)
 
 
 def test_dropout_does_not_write_the_state_that_it_reads():
