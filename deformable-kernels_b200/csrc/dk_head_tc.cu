@@ -11,8 +11,8 @@
 // 16-bit sums stay in TMEM, those of the logits up to 4096 features (kLongDepth).
 // fp32 operands are three bf16 pieces each (8 bits a piece, 24 in all).  A stage holds one piece of both; the six products of
 // pieces that reach 2^-24 are taken from three stages, that of the leading pieces into one accumulator, the five
-// small ones into another: the additions of the tensor cores cut, and a cut of the small sum costs nothing.  After every eight steps
-// the epilogue adds both to sums in registers, which round, so that no more than 32 cuts meet in one value.
+// small ones into another: the additions of the tensor cores cut, and a cut of the small sum costs nothing.  After every four steps
+// the epilogue adds both to sums in registers, which round, so that no more than 16 cuts meet in one value.
 //
 // Measured, one B200: logits with statistics 1.29 ms at 8192 x 2048 x 65536 (2.20 Tflop: 1.71 Pflop/s, tensor pipe 96 % of the
 // cycles), 0.146 at 4096 x 1280 x 21841 (1.57 Pflop/s, 87 %: 19 rounds of tiles, the last a half); with dz 0.174 (70 %: its 179 MB
@@ -37,7 +37,7 @@ using ring::smem_u32;
 namespace {
 
 __device__ int g_head_error;  // set when a bounded wait ran out
-// Nanoseconds.  The longest wait is the epilogue's for one sum in TMEM: 1024 steps of a gradient (split_products), 64 of the logits (kLongDepth), 8 of
+// Nanoseconds.  The longest wait is the epilogue's for one sum in TMEM: 1024 steps of a gradient (split_products), 64 of the logits (kLongDepth), 4 of
 // fp32 with six products each.  A step takes 0.235 us where nothing hides the loads' latency: a quarter of a millisecond.
 constexpr unsigned long long kWaitLimit = 2000000000;
 std::atomic<unsigned long long> g_wait_limit{kWaitLimit};
@@ -447,6 +447,10 @@ __device__ __forceinline__ void take_one(float* v, unsigned a, bool set) {
 // registers every 2048 (9e-7 at 16384); that costs up to a fifth of the time of many tiles (4096 rows, 4096 features, 21841 classes: loss 458 -> 540 us, step
 // 2.34 -> 2.49 ms; at 2560 features it would be 300 -> 355 and 1.43 -> 1.64), and 1 to 3 % of few (1024 x 16384 x 1000).
 constexpr int kLongDepth = 64, kLongChunk = 32;  // steps of 64 features
+// fp32: errors of dx and dw against fp64 as 32-bit products have them or smaller (256 x 1280 x 1000: 3.5e-7 and 3.4e-7, theirs 7.1e-7 and 5.1e-7; features of
+// one sign 4.7e-7 and 7.5e-7, theirs 4.7e-7 and 3.0e-7).  Every eight steps: 6.6e-7 and 3.7e-7, 6.6e-7 and 8.2e-7, losses near zero (4 x 2225 x 2) 1.6e-6 in
+// place of 4.8e-7, for 1 % less time; every two halves them again for 5 % more.
+constexpr int kPiecesChunk = 4;
 static_assert(kLongDepth >= kLongChunk, "the last sum is taken by itself: there is one before it");
 
 // LONG: many features, whose sums are added up in registers every kLongChunk steps
@@ -459,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_kernel(const __grid_constant
   constexpr int kWide = BN / kGroups;              // columns of an epilogue warp
   constexpr int kAcc = PIECES == 1 ? BN : 2 * BN;  // columns of an accumulator
   constexpr bool kTaken = PIECES > 1 || LONG;      // sums in registers
-  constexpr int kChunk = PIECES > 1 ? 8 : LONG ? kLongChunk : 1 << 30;  // steps between two takings of the accumulator
+  constexpr int kChunk = PIECES > 1 ? kPiecesChunk : LONG ? kLongChunk : 1 << 30;  // steps between two takings of the accumulator
   static_assert(PIECES == 1 || kWide == 64, "the sums of a row are 64 registers");
   static_assert(2 * kAcc <= 512, "two accumulators in TMEM");
   SharedTail& t = *reinterpret_cast<SharedTail*>(smem + kStages * kStage + 8 * kStageWarp);

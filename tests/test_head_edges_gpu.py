@@ -369,3 +369,21 @@ def test_features_in_the_millions():
         dz[torch.arange(rows), y] -= 1
         for a, c in ((dx, dz @ wd), (dw, dz.t() @ xd)):
             assert (a.double() - c).norm() <= (2.0 ** -7 + 4 * off) * c.norm()
+
+
+@pytest.mark.parametrize("rows, classes", [(9, 2), (40, 2), (200, 2), (200, 3000)])
+def test_fp32_sums_are_cut_no_more_than_sixteen_times(rows, classes):
+    """A one and then small products, one for every addition of the tensor cores, each a little less than the last bit of the sum so
+    far: a cut loses it whole.  Of 32 such additions sixteen may meet in one accumulator before sums that round take over;
+    the exact logit is 1 + 31 (255 / 256) 2^-23.  The loss of the other class, log(classes - 1 + e^z), moves by less than
+    the logit and is rounded in four places."""
+    x, w = torch.zeros(rows, 512), torch.zeros(classes, 512)
+    x[:, ::16], w[0, ::16] = 2.0 ** -11, 2.0 ** -12 * 255 / 256
+    x[:, 0], w[0, 0] = 1.0, 1.0
+    y = torch.ones(rows, dtype=torch.int64)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, w)]
+    loss = functions().linear_cross_entropy(leaves[0], leaves[1], y.to(DEV), reduction="none").detach().cpu().double()
+    z = 1 + 31 * (255 / 256) * 2.0 ** -23
+    want = torch.log(torch.tensor(classes - 1 + torch.exp(torch.tensor(z, dtype=torch.double)).item(), dtype=torch.double)).item()
+    share = torch.exp(torch.tensor(z, dtype=torch.double)).item() / torch.exp(torch.tensor(want, dtype=torch.double)).item()
+    assert ((loss - want).abs() <= share * 16 * 2.0 ** -23 + 4 * 2.0 ** -24 * want).all(), ((loss - want).abs().max().item() * 2 ** 23, share)
