@@ -7,8 +7,8 @@
 //   dx = dz W,   dW = dz^T x,   db = sum_t dz_t
 //
 // Forward: tiles of logits live in registers only; each leaves (maximum, sum of exponentials) of its rows, and a second
-// kernel joins the tiles of a row in fixed order.  Backward: a piece of the vocabulary at a time, the
-// logits of the piece once more, dz of the piece into the workspace, then the two products.
+// kernel joins the tiles of a row in fixed order.  Backward: a piece of the rows or of the classes at a time (all of
+// them, where dz is no larger than a piece), its logits once more, its dz into the workspace, then the two products.
 //
 // Here: the C entry points, the kernel that joins a row's tiles, and fp64 on the CUDA cores.  The other types: dk_head_tc.cu.
 #include <limits.h>

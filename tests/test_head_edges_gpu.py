@@ -387,3 +387,22 @@ def test_fp32_sums_are_cut_no_more_than_sixteen_times(rows, classes):
     want = torch.log(torch.tensor(classes - 1 + torch.exp(torch.tensor(z, dtype=torch.double)).item(), dtype=torch.double)).item()
     share = torch.exp(torch.tensor(z, dtype=torch.double)).item() / torch.exp(torch.tensor(want, dtype=torch.double)).item()
     assert ((loss - want).abs() <= share * 16 * 2.0 ** -23 + 4 * 2.0 ** -24 * want).all(), ((loss - want).abs().max().item() * 2 ** 23, share)
+
+
+@pytest.mark.parametrize("rows", [3, 60])
+@pytest.mark.parametrize("dtype", list(H.DTYPES))
+def test_weights_that_are_not_finite(dtype, rows):
+    """A logit of -inf takes its class out of the row; in fp32, whose pieces of an infinity are not finite, the loss may be NaN
+    instead.  +inf and NaN make NaN."""
+    x, w, y, b, _ = make(rows, 40, 30, dtype, seed=rows)
+    y[y == 7] = 8
+    out = torch.nn.functional.cross_entropy(*[(x.double() @ w.double().t() + b.double())[:, [i for i in range(30) if i != 7]], y - (y > 7).long()],
+                                            reduction="none")
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        w2 = w.clone()
+        w2[7, 11] = bad
+        loss = functions().linear_cross_entropy(x.to(DEV), w2.to(DEV), y.to(DEV), b.to(DEV), reduction="none").cpu().double()
+        gone = x[:, 11].double() * bad == float("-inf")
+        assert torch.isnan(loss[~gone]).all()
+        right = (loss - out).abs() < 1e-4 * (1 + out)
+        assert (right | (torch.isnan(loss) if dtype == "fp32" else torch.zeros_like(right)))[gone].all()
