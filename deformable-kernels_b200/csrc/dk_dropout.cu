@@ -223,6 +223,9 @@ __global__ void __launch_bounds__(256) dropout_runs_kernel(const T* __restrict__
 // Long runs (planes, samples) of a multiple of eight elements, both tensors on 16 bytes: a warp has up to kPart elements of one run, so that the division and the
 // counter are its own and not those of every eight elements (28.9 M fp32 values in planes of 3136, p = 0.2: 35 us, 5.9 TB/s, against 41).
 constexpr int kPart = 1024;
+// Runs from here on go that way; below, a warp has too little to do for its counter (67 M values, p = 0.2, us here / in dropout_runs_kernel: fp16 runs of 64
+// 383 / 81, 192 133 / 81, 256 101 / 81, 384 72 / 81, 1024 41 / 81; fp32 64 314 / 88, 192 112 / 88, 256 87 / 86, 384 78 / 86, 1024 76 / 86).
+constexpr unsigned long long kLongRun = 320;
 template <typename T, bool STATE>
 __global__ void __launch_bounds__(256) dropout_long_runs_kernel(const T* __restrict__ x, T* __restrict__ y, const DropArgs a, unsigned parts,
                                                                 unsigned long long units) {
@@ -262,7 +265,7 @@ int launch_dropout(const void* input, void* output, DropArgs a, cudaStream_t s) 
   T* y = (T*)output;
   const bool vector = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0;
   const unsigned most = (unsigned)device_sm_count() * 32;
-  if (vector && a.run >= 256 && a.run % 8 == 0) {
+  if (vector && a.run >= kLongRun && a.run % 8 == 0) {
     const unsigned long long parts = (a.run + kPart - 1) / kPart, units = a.count / a.run * parts;
     if (a.count % a.run == 0 && parts <= 0xffffffffull) {
       a.small = units <= 0xffffffffull;

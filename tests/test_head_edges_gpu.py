@@ -406,3 +406,10 @@ def test_weights_that_are_not_finite(dtype, rows):
         assert torch.isnan(loss[~gone]).all()
         right = (loss - out).abs() < 1e-4 * (1 + out)
         assert (right | (torch.isnan(loss) if dtype == "fp32" else torch.zeros_like(right)))[gone].all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "fp32", "fp64"])
+def test_dropout_of_runs_on_both_sides_of_the_rule(dtype):
+    for run in (8, 248, 256, 312, 320, 328, 384, 1016, 1024, 1032, 2056):
+        x = torch.randn(37, run, generator=torch.Generator().manual_seed(run)).to(H.DTYPES[dtype])
+        assert torch.equal(functions().dropout(x.to(DEV), 0.3, 9, 2, shared_dims=1).cpu(), H.dropout(x, 0.3, 9, 2, 1))
