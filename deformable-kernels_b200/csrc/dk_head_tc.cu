@@ -1131,7 +1131,10 @@ void split_products(BackwardPlan& p, int D, int pieces) {
   const long long tiles_w = (long long)div_up(p.vc, bm) * tn, tiles_x = (long long)div_up(p.tc, bm) * tn;
   const int blocks_w = div_up(p.tc, kBox), blocks_x = div_up(p.vc, kBox);
   const long long total = tiles_w * blocks_w + tiles_x * blocks_x;
-  // at least 32 steps a split (of fp32, six products each, 8): the launch that joins the sums takes as long as some 20 steps
+  // at least 32 steps a split (of fp32, six products each, 8): the launch that joins the sums takes as long as some 20 steps.  Steps of training as
+  // graphs, bf16, with at least 16 / 32 / 64, us: 1024 rows of 1280 features, 1000 classes 38 / 38 / 38 (8: 51), 2048 x 256 x 4096 57 / 51 / 54, 25088 x 256 x 150
+  // 53 / 51 / 55, 100 x 264 x 11000 37 / 41 / 49, 4096 x 256 x 150 29 / 33 / 37, 9000 x 64 x 40 27 / 31 / 35; fp32 with 4 / 8 / 16: 64 x 520 x 4099
+  // 63 / 64 / 70, 100 x 264 x 11000 70 / 69 / 75, 4096 x 256 x 150 45 / 47 / 55
   const int least = pieces == 1 ? 32 : 8;
   // and of 16-bit types at most 1024, 4096 additions that cut: 2^-12 of a sum of one sign, half of what fp16 rounds.  Parts of sums are rounded additions; they
   // take 8 KB of scratch a feature at most (a piece has 2^27 values of dz).
@@ -1147,8 +1150,9 @@ void split_products(BackwardPlan& p, int D, int pieces) {
 
 // the rounds of the two products' items that let all clusters end at about the same time
 Schedule schedule_of(const Product& dw, const Product& dx, int clusters, int pieces) {
-  // a tile takes the epilogue as long as it takes the tensor cores ten steps (six products a step: two); without that 64 rows, 32768 classes of 1280
-  // features, whose dw tiles are one step, take 264 us instead of 126
+  // a tile takes the epilogue as long as it takes the tensor cores ten steps (six products a step: two).  Steps of training as graphs, bf16, counted as at
+  // least 1 / 5 / 10 / 20 steps, us: 64 rows of 1280 features, 32768 classes, whose dw tiles are one step, 176 / 103 / 103 / 106, 25088 x 256 x 150 51 / 51 / 51 / 53,
+  // 65536 x 256 x 21 69 / 69 / 70 / 72; fp32, 1 / 2 / 4: the first 443 / 414 / 421, the last 245 / 204 / 194
   const int least = pieces == 1 ? 10 : 2;
   const int n_w = dw.tiles_m * dw.tiles_n * dw.splits, n_x = dx.tiles_m * dx.tiles_n * dx.splits;
   Schedule c = {};
