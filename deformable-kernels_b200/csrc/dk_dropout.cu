@@ -7,8 +7,8 @@
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011) with the seed as key
 // and (j / 8, offset) as counter gives the upper 16 bits of eight draws at once; their lower 16 bits come from the counter
 // with the highest bit of j / 8 set, and only a draw whose upper half equals the threshold's (one of 65536) looks at them.
-// With 32 bits of one word per element the generator, not memory, is the bound: 142 us against 106 for 154 M fp16 values
-// (308 MB in, 308 MB out, 5.8 TB/s; a copy of them takes 96).
+// With 32 bits of one word per element the generator, not memory, is the bound: 142 us against 109 for 154 M fp16 values
+// (308 MB in, 308 MB out, 5.7 TB/s; a copy of them takes 96).
 //
 // A dropped element is zero whatever x holds there (infinities and NaN included).  x / (1 - p) is a product with the fp32
 // (fp64) reciprocal, rounded once to the tensor's type.
@@ -36,7 +36,7 @@ struct Key {
 };
 
 // The generator's key, kept for the backward where that is wanted.  As 32-bit words that are loaded without a condition it stays in
-// uniform registers, its ten round keys with it: 104 us against 127 (154 M fp16 values).
+// uniform registers, its ten round keys with it: 18 % less time (154 M fp16 values).
 template <bool STATE>
 __device__ __forceinline__ Key key_of(const DropArgs& a) {
   const unsigned add0 = (unsigned)a.offset, add1 = (unsigned)(a.offset >> 32);
@@ -151,7 +151,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 times<__nv_bfloat16, float>
 
 // Every element has its own draw; both tensors begin on 16 bytes, hold whole groups of eight (the elements of this launch), and the
 // threshold's upper half is below 0xffff.  A thread takes eight elements at a time, one counter's worth of draws.  All the warps an SM can hold, with registers to
-// match, hide the generator's latency: 102 us against 123 with the registers that ptxas takes by itself.
+// match, hide the generator's latency: 17 % less time than with the registers that ptxas takes by itself.
 template <typename T, bool STATE>
 __global__ void __launch_bounds__(256, 8) dropout_kernel(const T* __restrict__ x, T* __restrict__ y, const DropArgs a) {
   constexpr int kPieces = 8 * sizeof(T) / 16;
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(256) dropout_runs_kernel(const T* __restrict__
 }
 
 // Long runs (planes, samples) of a multiple of eight elements, both tensors on 16 bytes: a warp has up to kPart elements of one run, so that the division and the
-// counter are its own and not those of every eight elements (28.9 M fp32 values in planes of 3136, p = 0.2: 35 us, 5.9 TB/s, against 41).
+// counter are its own and not those of every eight elements (28.9 M fp32 values in planes of 3136, p = 0.2: 37 us against 41).
 constexpr int kPart = 1024;
 // Runs from here on go that way; below, a warp has too little to do for its counter (67 M values, p = 0.2, us here / in dropout_runs_kernel: fp16 runs of 64
 // 383 / 81, 192 133 / 81, 256 101 / 81, 384 72 / 81, 1024 41 / 81; fp32 64 314 / 88, 192 112 / 88, 256 87 / 86, 384 78 / 86, 1024 76 / 86).
